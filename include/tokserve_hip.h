@@ -2,7 +2,8 @@
  * tokserve_hip.h -- C ABI of libtokserve_hip.so, the MI355X (gfx950) kernels of
  * tokserve's continuous-batching hot path: KV append into paged blocks, block
  * table gathers, paged attention (decode and chunked prefill), RMSNorm, RoPE
- * greedy token selection and the elementwise vector_add.
+ * greedy token selection and the elementwise vector_add; and MXFP4, 4-bit K/V
+ * pools and products with 4-bit weights.
  *
  * Conventions shared by every entry point
  *   - All pointers are device pointers (HBM), except where a comment says host.
@@ -53,7 +54,7 @@ enum tks_status {
 };
 
 /* ABI version of this header; bumped on any signature change. */
-#define TKS_ABI_VERSION 12
+#define TKS_ABI_VERSION 13
 int32_t tks_abi_version(void);
 
 /* Static description of a status code (never NULL). */
@@ -414,6 +415,134 @@ int32_t tks_rope_append_paged_decode_fp8_rows(
     int32_t max_seq_len, float scale, int32_t pages_per_split, void *out,
     int64_t out_seq_stride, int64_t out_head_stride, void *workspace, int64_t workspace_bytes,
     int32_t dtype, tks_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * MXFP4 (OCP microscaled 4-bit floating point). No counterpart in the reference,
+ * whose weights and caches have the model dtype. 32 consecutive values x of a row
+ * are a block of 17 bytes, held apart as codes and scales:
+ *   scale = 2^(E - 127), E = clamp(e - 2, 2, 252), e the biased fp32 exponent of
+ *           the block's largest |x| (0 for zeros and fp32 subnormals): one e8m0 byte
+ *   code  = e2m1(x / scale): 0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign, rounded to
+ *           nearest with ties to the even code, at most 6: four bits, two codes to
+ *           a byte, the even element in the low nibble
+ *   a block with a NaN or an infinity: E = 255 and codes 0; it reads back as NaN
+ *   decoded = code * scale
+ * Codes and scales are contiguous: (rows, cols / 2) and (rows, cols / 32) bytes;
+ * cols must be a multiple of 32. Codes passed to products are 16-byte aligned, to
+ * the quantisation and back 4-byte.
+ */
+/* Rows (rows, cols) of `dtype`, stride input_row_stride, to codes and scales. */
+int32_t tks_mxfp4_quantize(const void *input, int64_t input_row_stride, int64_t num_rows,
+                           int64_t num_cols, void *codes, void *scales, int32_t dtype,
+                           tks_stream_t stream);
+
+/* Codes and scales to rows of `dtype`, rounded once to it. */
+int32_t tks_mxfp4_dequantize(const void *codes, const void *scales, int64_t num_rows,
+                             int64_t num_cols, void *out, int64_t out_row_stride, int32_t dtype,
+                             tks_stream_t stream);
+
+/* out[m, n] = sum_k A[m, k] B[n, k] over MXFP4 matrices A (num_rows, depth) and B
+ * (num_cols, depth), summed in fp32 and rounded once to `dtype`; results do not
+ * change from run to run. The workspace (16-byte aligned, of the size that
+ * tks_mxfp4_matmul_workspace_bytes gives for the shape; 0: may be NULL) needs no
+ * initial contents; launches sharing it must be stream-ordered. */
+int64_t tks_mxfp4_matmul_workspace_bytes(int64_t num_rows, int64_t num_cols, int64_t depth);
+
+int32_t tks_mxfp4_matmul(const void *a_codes, const void *a_scales, const void *b_codes,
+                         const void *b_scales, int64_t num_rows, int64_t num_cols, int64_t depth,
+                         void *out, int64_t out_row_stride, void *workspace,
+                         int64_t workspace_bytes, int32_t dtype, tks_stream_t stream);
+
+/* A projection with MXFP4 weights: rows of `dtype` are quantized as
+ * tks_mxfp4_quantize does and multiplied as tks_mxfp4_matmul does; same results as
+ * the two calls. Workspace as for the product, from its own size query. */
+int64_t tks_mxfp4_linear_workspace_bytes(int64_t num_rows, int64_t num_cols, int64_t depth);
+
+int32_t tks_mxfp4_linear(const void *input, int64_t input_row_stride, const void *weight_codes,
+                         const void *weight_scales, int64_t num_rows, int64_t num_cols,
+                         int64_t depth, void *out, int64_t out_row_stride, void *workspace,
+                         int64_t workspace_bytes, int32_t dtype, tks_stream_t stream);
+
+/* K/V pools in MXFP4 (a pool-layout variant behind PagedKVStorage, as the fp8
+ * pools are): codes [L, NB, Hkv, BS, Dh / 2] and scale bytes [L, NB, Hkv, BS,
+ * Dh / 32], blocks along Dh, which must be 32, 64, 96 or 128; pools 16-byte aligned.
+ * `head_dim` is Dh. Each entry takes the arguments of its *_fp8_rows counterpart
+ * with the scale bytes in place of the fp32 scales; `dtype` is the type of the other
+ * tensors (new rows, gathered rows, query, output). Rows no sequence has written
+ * are never read into an output. */
+int32_t tks_kv_append_mxfp4(const void *key, int64_t key_token_stride, int64_t key_head_stride,
+                            const void *value, int64_t value_token_stride,
+                            int64_t value_head_stride, int64_t num_tokens, void *key_cache,
+                            void *value_cache, void *k_scales, void *v_scales, int32_t num_layers,
+                            int64_t num_blocks, int32_t num_kv_heads, int32_t block_size,
+                            int32_t head_dim, int32_t layer_index, const int64_t *slot_mapping,
+                            int32_t dtype, tks_stream_t stream);
+
+/* Gathered rows are the decoded values rounded once to `dtype`. */
+int32_t tks_paged_gather_mxfp4(const void *key_cache, const void *value_cache,
+                               const void *k_scales, const void *v_scales, int32_t num_layers,
+                               int64_t num_blocks, int32_t num_kv_heads, int32_t block_size,
+                               int32_t head_dim, int32_t layer_index, const int32_t *block_tables,
+                               int32_t block_table_stride, const int32_t *seq_lens,
+                               const int32_t *cu_seqlens, int32_t num_seqs, int32_t max_seq_len,
+                               void *key_out, void *value_out, int64_t out_token_stride,
+                               int64_t out_head_stride, int32_t dtype, tks_stream_t stream);
+
+/* tks_rope then tks_kv_append_mxfp4 of the rotated keys, in one launch. */
+int32_t tks_rope_kv_append_mxfp4(
+    const void *query, void *query_out, int64_t q_ts, int64_t q_hs, int64_t qo_ts, int64_t qo_hs,
+    int32_t num_q_heads, const void *key, void *key_out, int64_t k_ts, int64_t k_hs, int64_t ko_ts,
+    int64_t ko_hs, const void *value, int64_t v_ts, int64_t v_hs, int32_t num_kv_heads,
+    int64_t num_tokens, int32_t head_dim, const int64_t *positions, const void *cos_cache,
+    const void *sin_cache, int64_t cache_len, void *key_cache, void *value_cache, void *k_scales,
+    void *v_scales, int32_t num_layers, int64_t num_blocks, int32_t block_size,
+    int32_t layer_index, const int64_t *slot_mapping, int32_t dtype, tks_stream_t stream);
+
+/* Decode attention: the function of tks_paged_attention_decode on the decoded pools
+ * (exact values, products and sums in fp32). At most 16 query heads to a KV head.
+ * Workspace of tks_paged_attention_decode_workspace_bytes. */
+int32_t tks_paged_attention_decode_mxfp4(
+    const void *query, int64_t q_seq_stride, int64_t q_head_stride, const void *key_cache,
+    const void *value_cache, const void *k_scales, const void *v_scales, int32_t num_layers,
+    int64_t num_blocks, int32_t num_kv_heads, int32_t block_size, int32_t head_dim,
+    int32_t layer_index, const int32_t *block_tables, int32_t block_table_stride,
+    const int32_t *seq_lens, const int32_t *seq_order, int32_t num_seqs, int32_t num_q_heads,
+    int32_t max_seq_len, float scale, int32_t pages_per_split, void *out, int64_t out_seq_stride,
+    int64_t out_head_stride, void *workspace, int64_t workspace_bytes, int32_t dtype,
+    tks_stream_t stream);
+
+/* tks_rope_kv_append_mxfp4 then tks_paged_attention_decode_mxfp4, the rotated queries
+ * staged in `out`. */
+int32_t tks_rope_append_paged_decode_mxfp4(
+    const void *query, int64_t q_seq_stride, int64_t q_head_stride, const void *key,
+    int64_t k_seq_stride, int64_t k_head_stride, const void *value, int64_t v_seq_stride,
+    int64_t v_head_stride, const int64_t *positions, const void *cos_cache, const void *sin_cache,
+    int64_t cache_len, const int64_t *slot_mapping, void *key_cache, void *value_cache,
+    void *k_scales, void *v_scales, int32_t num_layers, int64_t num_blocks, int32_t num_kv_heads,
+    int32_t block_size, int32_t head_dim, int32_t layer_index, const int32_t *block_tables,
+    int32_t block_table_stride, const int32_t *seq_lens, const int32_t *seq_order,
+    int32_t num_seqs, int32_t num_q_heads, int32_t max_seq_len, float scale,
+    int32_t pages_per_split, void *out, int64_t out_seq_stride, int64_t out_head_stride,
+    void *workspace, int64_t workspace_bytes, int32_t dtype, tks_stream_t stream);
+
+/* Chunked-prefill attention: the pages the batch reads are decoded into the
+ * workspace (a dense pool in `dtype` of ceil(max_seq_len / block_size) pages to a
+ * sequence, values rounded once to it, and its identity block table; 16-byte aligned),
+ * which tks_paged_attention_prefill then reads. */
+int64_t tks_paged_attention_prefill_mxfp4_workspace_bytes(int32_t num_seqs, int32_t num_kv_heads,
+                                                          int32_t head_dim, int32_t block_size,
+                                                          int32_t max_seq_len, int32_t dtype);
+
+int32_t tks_paged_attention_prefill_mxfp4(
+    const void *query, int64_t q_token_stride, int64_t q_head_stride, const void *key_cache,
+    const void *value_cache, const void *k_scales, const void *v_scales, int32_t num_layers,
+    int64_t num_blocks, int32_t num_kv_heads, int32_t block_size, int32_t head_dim,
+    int32_t layer_index, const int32_t *block_tables, int32_t block_table_stride,
+    const int32_t *seq_lens, const int32_t *cu_seqlens_q, const int32_t *seq_order,
+    int32_t num_seqs, int64_t num_tokens, int32_t num_q_heads, int32_t max_query_len,
+    int32_t max_seq_len, float scale, void *out, int64_t out_token_stride,
+    int64_t out_head_stride, void *workspace, int64_t workspace_bytes, int32_t dtype,
+    tks_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * RMSNorm over the last dimension.

@@ -19,6 +19,7 @@
 // (m, l, acc) then go to the caller's workspace and merge_splits_kernel, a
 // second launch, combines them. Large batches run as one launch.
 #include "attention_common.hpp"
+#include "mxfp4_kv.hpp"
 
 #include <algorithm>
 #include <atomic>
@@ -571,6 +572,27 @@ struct RopeAppend {
   const int64_t *slot_mapping;
 };
 
+// The second launch of a split decode.
+int32_t launch_merge(const int32_t *seq_lens, int32_t key_cap, int32_t block_size, int32_t pps,
+                     int32_t max_splits, int32_t num_seqs, int32_t num_q_heads, int32_t head_dim,
+                     const Workspace &w, void *out, int64_t out_seq_stride,
+                     int64_t out_head_stride, int32_t dtype, hipStream_t s) {
+  const dim3 grid(num_q_heads, num_seqs);
+  const int threads = head_dim > 64 ? 128 : 64;  // one thread per output element
+#define TKS_MERGE(TYPE)                                                                         \
+  merge_splits_kernel<TYPE><<<grid, threads, 0, s>>>(seq_lens, key_cap, block_size, pps,        \
+                                                     max_splits, num_q_heads, head_dim, w.m, w.l, \
+                                                     w.acc, static_cast<TYPE *>(out),             \
+                                                     out_seq_stride, out_head_stride)
+  switch (dtype) {
+    case TKS_FLOAT32: TKS_MERGE(float); break;
+    case TKS_FLOAT16: TKS_MERGE(_Float16); break;
+    default: TKS_MERGE(bf16_t); break;
+  }
+#undef TKS_MERGE
+  return check_launch();
+}
+
 int32_t decode_impl(const void *query, int64_t q_seq_stride, int64_t q_head_stride,
                     const void *key_cache, const void *value_cache, int32_t num_layers,
                     int64_t num_blocks, int32_t num_kv_heads, int32_t block_size,
@@ -729,20 +751,8 @@ int32_t decode_impl(const void *query, int64_t q_seq_stride, int64_t q_head_stri
     st = launch_generic(a, dtype, num_seqs, num_kv_heads, fp8_pools, s);
   }
   if (st != TKS_OK || splits == 1) return st;
-  const dim3 grid(num_q_heads, num_seqs);
-  const int threads = head_dim > 64 ? 128 : 64;  // one thread per output element
-#define TKS_MERGE(TYPE)                                                                         \
-  merge_splits_kernel<TYPE><<<grid, threads, 0, s>>>(seq_lens, key_cap, block_size, pps,        \
-                                                     max_splits, num_q_heads, head_dim, w.m, w.l, \
-                                                     w.acc, static_cast<TYPE *>(out),             \
-                                                     out_seq_stride, out_head_stride)
-  switch (dtype) {
-    case TKS_FLOAT32: TKS_MERGE(float); break;
-    case TKS_FLOAT16: TKS_MERGE(_Float16); break;
-    default: TKS_MERGE(bf16_t); break;
-  }
-#undef TKS_MERGE
-  return check_launch();
+  return launch_merge(seq_lens, key_cap, block_size, pps, max_splits, num_seqs, num_q_heads,
+                      head_dim, w, out, out_seq_stride, out_head_stride, dtype, s);
 }
 
 int32_t prefill_impl(const void *query, int64_t q_token_stride, int64_t q_head_stride,
@@ -1168,4 +1178,192 @@ extern "C" int32_t tks_rope_append_paged_decode_fp8_rows(
                      block_table_stride, seq_lens, seq_order, num_seqs, num_q_heads, max_seq_len,
                      scale, pages_per_split, out, out_seq_stride, out_head_stride, workspace,
                      workspace_bytes, true, 1.f, 1.f, dtype, stream, &ra, k_scales, v_scales);
+}
+
+// ------------------------------------------------------------------------
+// MXFP4 pools (mxfp4_kv.hpp): decode through decode_mxfp4.hip and the split merge above;
+// prefill over the pages decoded into a scratch pool of the query's dtype.
+// ------------------------------------------------------------------------
+
+namespace {
+
+int32_t decode_mxfp4_impl(const void *query, int64_t q_seq_stride, int64_t q_head_stride,
+                          const void *key_cache, const void *value_cache, const void *k_scales,
+                          const void *v_scales, int32_t num_layers, int64_t num_blocks,
+                          int32_t num_kv_heads, int32_t block_size, int32_t head_dim,
+                          int32_t layer_index, const int32_t *block_tables,
+                          int32_t block_table_stride, const int32_t *seq_lens,
+                          const int32_t *seq_order, int32_t num_seqs, int32_t num_q_heads,
+                          int32_t max_seq_len, float scale, int32_t pages_per_split, void *out,
+                          int64_t out_seq_stride, int64_t out_head_stride, void *workspace,
+                          int64_t workspace_bytes, int32_t dtype, tks_stream_t stream) {
+  if (!valid_dtype(dtype)) return TKS_ERR_TYPE;
+  if (!mx_pool_ok(num_layers, num_blocks, num_kv_heads, block_size, head_dim) || num_seqs < 0 ||
+      num_q_heads <= 0 || num_q_heads % num_kv_heads != 0 || max_seq_len < 0 ||
+      pages_per_split < 0 || num_q_heads / num_kv_heads > kGenMaxG)
+    return TKS_ERR_VALUE;
+  if (layer_index < 0 || layer_index >= num_layers) return TKS_ERR_INDEX;
+  if (num_seqs == 0) return TKS_OK;
+  if (num_seqs > 65535 || ceil_div(max_seq_len, block_size) > block_table_stride)
+    return TKS_ERR_VALUE;
+  if (!query || !mx_pools_given(key_cache, value_cache, k_scales, v_scales) || !block_tables ||
+      !seq_lens || !out)
+    return TKS_ERR_VALUE;
+  const int32_t pps = choose_pages_per_split(num_seqs, num_kv_heads, block_size, max_seq_len,
+                                             pages_per_split, split_unit(block_size));
+  const int32_t max_splits = split_count(max_seq_len, block_size, pps);
+  if (max_splits > kMaxGridSplits) return TKS_ERR_VALUE;
+  const Workspace w = carve(workspace, num_seqs, num_q_heads, max_splits, head_dim);
+  if (max_splits > 1 && (workspace == nullptr || workspace_bytes < w.bytes))
+    return TKS_ERR_WORKSPACE;
+  const int64_t split_keys = static_cast<int64_t>(pps) * block_size;
+  const int32_t key_cap = static_cast<int32_t>(std::min<int64_t>(
+      std::min<int64_t>(block_table_stride, static_cast<int64_t>(max_splits) * pps) * block_size,
+      INT32_MAX - 64));
+  MxDecodeArgs a{};
+  a.q = query;
+  a.q_ss = q_seq_stride;
+  a.q_hs = q_head_stride;
+  a.kc = mx_pool(const_cast<void *>(key_cache), const_cast<void *>(k_scales), num_blocks,
+                 num_kv_heads, block_size, head_dim, layer_index);
+  a.vc = mx_pool(const_cast<void *>(value_cache), const_cast<void *>(v_scales), num_blocks,
+                 num_kv_heads, block_size, head_dim, layer_index);
+  a.bt = block_tables;
+  a.bt_stride = block_table_stride;
+  a.seq_lens = seq_lens;
+  a.seq_order = seq_order;
+  a.num_q_heads = num_q_heads;
+  a.group = num_q_heads / num_kv_heads;
+  a.scale_log2 = scale * kLog2e;
+  a.split_keys = static_cast<int32_t>(std::min<int64_t>(split_keys, INT32_MAX - 64));
+  a.max_splits = max_splits;
+  a.key_cap = key_cap;
+  a.out = out;
+  a.o_ss = out_seq_stride;
+  a.o_hs = out_head_stride;
+  a.ws_m = w.m;
+  a.ws_l = w.l;
+  a.ws_acc = w.acc;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int32_t st = launch_decode_mxfp4(a, dtype, num_seqs, s);
+  if (st != TKS_OK || max_splits == 1) return st;
+  return launch_merge(seq_lens, key_cap, block_size, pps, max_splits, num_seqs, num_q_heads,
+                      head_dim, w, out, out_seq_stride, out_head_stride, dtype, s);
+}
+
+}  // namespace
+
+extern "C" int32_t tks_paged_attention_decode_mxfp4(
+    const void *query, int64_t q_seq_stride, int64_t q_head_stride, const void *key_cache,
+    const void *value_cache, const void *k_scales, const void *v_scales, int32_t num_layers,
+    int64_t num_blocks, int32_t num_kv_heads, int32_t block_size, int32_t head_dim,
+    int32_t layer_index, const int32_t *block_tables, int32_t block_table_stride,
+    const int32_t *seq_lens, const int32_t *seq_order, int32_t num_seqs, int32_t num_q_heads,
+    int32_t max_seq_len, float scale, int32_t pages_per_split, void *out, int64_t out_seq_stride,
+    int64_t out_head_stride, void *workspace, int64_t workspace_bytes, int32_t dtype,
+    tks_stream_t stream) {
+  return decode_mxfp4_impl(query, q_seq_stride, q_head_stride, key_cache, value_cache, k_scales,
+                           v_scales, num_layers, num_blocks, num_kv_heads, block_size, head_dim,
+                           layer_index, block_tables, block_table_stride, seq_lens, seq_order,
+                           num_seqs, num_q_heads, max_seq_len, scale, pages_per_split, out,
+                           out_seq_stride, out_head_stride, workspace, workspace_bytes, dtype,
+                           stream);
+}
+
+extern "C" int32_t tks_rope_append_paged_decode_mxfp4(
+    const void *query, int64_t q_seq_stride, int64_t q_head_stride, const void *key,
+    int64_t k_seq_stride, int64_t k_head_stride, const void *value, int64_t v_seq_stride,
+    int64_t v_head_stride, const int64_t *positions, const void *cos_cache, const void *sin_cache,
+    int64_t cache_len, const int64_t *slot_mapping, void *key_cache, void *value_cache,
+    void *k_scales, void *v_scales, int32_t num_layers, int64_t num_blocks, int32_t num_kv_heads,
+    int32_t block_size, int32_t head_dim, int32_t layer_index, const int32_t *block_tables,
+    int32_t block_table_stride, const int32_t *seq_lens, const int32_t *seq_order,
+    int32_t num_seqs, int32_t num_q_heads, int32_t max_seq_len, float scale,
+    int32_t pages_per_split, void *out, int64_t out_seq_stride, int64_t out_head_stride,
+    void *workspace, int64_t workspace_bytes, int32_t dtype, tks_stream_t stream) {
+  // Every refusal of the attention comes before the append writes anything.
+  if (max_seq_len < 0 || pages_per_split < 0 || num_kv_heads <= 0 || num_q_heads <= 0 ||
+      num_q_heads % num_kv_heads != 0 || num_q_heads / num_kv_heads > kGenMaxG ||
+      block_size <= 0 || num_seqs < 0 || num_seqs > 65535 ||
+      ceil_div(max_seq_len, block_size) > block_table_stride)
+    return valid_dtype(dtype) ? TKS_ERR_VALUE : TKS_ERR_TYPE;
+  if (num_seqs > 0 && (!block_tables || !seq_lens || !out)) return TKS_ERR_VALUE;
+  const int64_t needed = tks_paged_attention_decode_workspace_bytes(
+      num_seqs, num_q_heads, num_kv_heads, head_dim, block_size, max_seq_len, pages_per_split);
+  if (needed < 0) return TKS_ERR_VALUE;
+  if (needed > 0 && (workspace == nullptr || workspace_bytes < needed)) return TKS_ERR_WORKSPACE;
+  // The rotated queries are staged in `out`, which each workgroup reads before it, or the
+  // merge, writes its rows.
+  const int32_t st = tks_rope_kv_append_mxfp4(
+      query, out, q_seq_stride, q_head_stride, out_seq_stride, out_head_stride, num_q_heads, key,
+      nullptr, k_seq_stride, k_head_stride, 0, 0, value, v_seq_stride, v_head_stride,
+      num_kv_heads, num_seqs, head_dim, positions, cos_cache, sin_cache, cache_len, key_cache,
+      value_cache, k_scales, v_scales, num_layers, num_blocks, block_size, layer_index,
+      slot_mapping, dtype, stream);
+  if (st != TKS_OK) return st;
+  return decode_mxfp4_impl(out, out_seq_stride, out_head_stride, key_cache, value_cache, k_scales,
+                           v_scales, num_layers, num_blocks, num_kv_heads, block_size, head_dim,
+                           layer_index, block_tables, block_table_stride, seq_lens, seq_order,
+                           num_seqs, num_q_heads, max_seq_len, scale, pages_per_split, out,
+                           out_seq_stride, out_head_stride, workspace, workspace_bytes, dtype,
+                           stream);
+}
+
+extern "C" int64_t tks_paged_attention_prefill_mxfp4_workspace_bytes(
+    int32_t num_seqs, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+    int32_t max_seq_len, int32_t dtype) {
+  if (!valid_dtype(dtype) || num_seqs < 0 || num_kv_heads <= 0 || head_dim <= 0 ||
+      block_size <= 0 || max_seq_len < 0)
+    return -1;
+  return mx_carve_pages(nullptr, num_seqs,
+                        static_cast<int32_t>(ceil_div(std::max(max_seq_len, 1), block_size)),
+                        num_kv_heads,
+                        block_size, head_dim, dtype)
+      .bytes;
+}
+
+extern "C" int32_t tks_paged_attention_prefill_mxfp4(
+    const void *query, int64_t q_token_stride, int64_t q_head_stride, const void *key_cache,
+    const void *value_cache, const void *k_scales, const void *v_scales, int32_t num_layers,
+    int64_t num_blocks, int32_t num_kv_heads, int32_t block_size, int32_t head_dim,
+    int32_t layer_index, const int32_t *block_tables, int32_t block_table_stride,
+    const int32_t *seq_lens, const int32_t *cu_seqlens_q, const int32_t *seq_order,
+    int32_t num_seqs, int64_t num_tokens, int32_t num_q_heads, int32_t max_query_len,
+    int32_t max_seq_len, float scale, void *out, int64_t out_token_stride,
+    int64_t out_head_stride, void *workspace, int64_t workspace_bytes, int32_t dtype,
+    tks_stream_t stream) {
+  if (!valid_dtype(dtype)) return TKS_ERR_TYPE;
+  if (!mx_pool_ok(num_layers, num_blocks, num_kv_heads, block_size, head_dim) || num_seqs < 0 ||
+      num_tokens < 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads != 0 ||
+      num_q_heads / num_kv_heads > kGenMaxG || max_query_len < 0 || max_seq_len < 0 ||
+      max_query_len > max_seq_len || block_table_stride < 0)
+    return TKS_ERR_VALUE;
+  if (layer_index < 0 || layer_index >= num_layers) return TKS_ERR_INDEX;
+  if (num_seqs == 0 || num_tokens == 0) return TKS_OK;
+  if (num_tokens > 0x7fffffff || ceil_div(max_seq_len, block_size) > block_table_stride)
+    return TKS_ERR_VALUE;
+  // (Queries of no keys: one page, of which nothing is read.)
+  const int32_t width = static_cast<int32_t>(ceil_div(std::max(max_seq_len, 1), block_size));
+  if (static_cast<int64_t>(num_seqs) * width > INT32_MAX) return TKS_ERR_VALUE;
+  if (!query || !mx_pools_given(key_cache, value_cache, k_scales, v_scales) || !block_tables ||
+      !seq_lens || !cu_seqlens_q || !out)
+    return TKS_ERR_VALUE;
+  const MxScratch sp = mx_carve_pages(workspace, num_seqs, width, num_kv_heads, block_size,
+                                      head_dim, dtype);
+  if (workspace == nullptr || workspace_bytes < sp.bytes || !aligned16(workspace))
+    return TKS_ERR_WORKSPACE;
+  const MxPool kc = mx_pool(const_cast<void *>(key_cache), const_cast<void *>(k_scales),
+                            num_blocks, num_kv_heads, block_size, head_dim, layer_index);
+  const MxPool vc = mx_pool(const_cast<void *>(value_cache), const_cast<void *>(v_scales),
+                            num_blocks, num_kv_heads, block_size, head_dim, layer_index);
+  const int32_t st =
+      launch_decode_mx_pages(kc, vc, block_tables, block_table_stride, seq_lens, num_seqs, width,
+                             sp, dtype, static_cast<hipStream_t>(stream));
+  if (st != TKS_OK) return st;
+  return prefill_impl(query, q_token_stride, q_head_stride, sp.k, sp.v, 1,
+                      static_cast<int64_t>(num_seqs) * width, num_kv_heads,
+                      block_size, head_dim, 0, sp.table, width, seq_lens,
+                      cu_seqlens_q, seq_order, num_seqs, num_tokens, num_q_heads, max_query_len,
+                      max_seq_len, scale, out, out_token_stride, out_head_stride, false, nullptr,
+                      0, 1.f, 1.f, dtype, stream);
 }

@@ -19,6 +19,7 @@
 #include <torch/headeronly/version.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
 #include <dlfcn.h>
@@ -51,9 +52,28 @@ using OptTensor = std::optional<Tensor>;
   X(tks_rope_kv_append)                  \
   X(tks_rope_kv_append_fp8)              \
   X(tks_rope_kv_append_fp8_rows)         \
+  X(tks_kv_append)                       \
+  X(tks_kv_append_fp8)                   \
+  X(tks_kv_append_fp8_rows)              \
+  X(tks_kv_append_mxfp4)                 \
+  X(tks_paged_gather)                    \
+  X(tks_paged_gather_fp8)                \
+  X(tks_paged_gather_fp8_rows)           \
+  X(tks_paged_gather_mxfp4)              \
   X(tks_rms_norm)                        \
   X(tks_argmax)                          \
-  X(tks_silu_mul)
+  X(tks_silu_mul)                        \
+  X(tks_mxfp4_quantize)                  \
+  X(tks_mxfp4_dequantize)                \
+  X(tks_mxfp4_matmul_workspace_bytes)    \
+  X(tks_mxfp4_matmul)                    \
+  X(tks_mxfp4_linear_workspace_bytes)    \
+  X(tks_mxfp4_linear)                    \
+  X(tks_paged_attention_decode_mxfp4)    \
+  X(tks_paged_attention_prefill_mxfp4_workspace_bytes) \
+  X(tks_paged_attention_prefill_mxfp4)   \
+  X(tks_rope_append_paged_decode_mxfp4)  \
+  X(tks_rope_kv_append_mxfp4)
 
 struct Library {
 #define TKS_FIELD(name) decltype(&::name) name = nullptr;
@@ -139,6 +159,9 @@ template <typename T>
 T *as(const OptTensor &t) { return static_cast<T *>(mut(t)); }
 int32_t i32(int64_t x) { return static_cast<int32_t>(x); }
 bool fp8(const Tensor &pool) { return pool.scalar_type() == at::kFloat8_e4m3fn; }
+// MXFP4 pools hold two codes to an element.
+bool mxfp4(const Tensor &pool) { return pool.scalar_type() == at::kFloat4_e2m1fn_x2; }
+int32_t head_dim(const Tensor &pool) { return i32(pool.size(4) * (mxfp4(pool) ? 2 : 1)); }
 
 // Scratch memory of one call, undefined for 0 bytes: from the caching allocator on the
 // launch's stream, so no other call, stream or thread shares it.
@@ -152,7 +175,7 @@ Tensor decode_workspace(const OptTensor &given, const Tensor &query, const Tenso
                         int64_t max_seq_len, int64_t pages_per_split) {
   if (given) return *given;
   return scratch(library().tks_paged_attention_decode_workspace_bytes(
-                     i32(query.size(0)), i32(query.size(1)), i32(pool.size(2)), i32(pool.size(4)),
+                     i32(query.size(0)), i32(query.size(1)), i32(pool.size(2)), head_dim(pool),
                      i32(pool.size(3)), i32(max_seq_len), i32(pages_per_split)),
                  query, "decode");
 }
@@ -164,6 +187,7 @@ void paged_attention_decode(const Tensor &query, const Tensor &key_cache,
                             int64_t pages_per_split, double k_scale, double v_scale,
                             const Tensor &out, const OptTensor &workspace,
                             const OptTensor &k_scales, const OptTensor &v_scales) {
+  const c10::DeviceGuard guard(query.device());
   const Library &l = library();
   const Tensor ws = decode_workspace(workspace, query, key_cache, max_seq_len, pages_per_split);
   void *ws_ptr = ws.defined() ? ws.mutable_data_ptr() : nullptr;
@@ -175,7 +199,7 @@ void paged_attention_decode(const Tensor &query, const Tensor &key_cache,
           return entry(query.const_data_ptr(), query.stride(0), query.stride(1),
                        kc.const_data_ptr(), value_cache.const_data_ptr(), rows...,
                        i32(kc.size(0)), kc.size(1), i32(kc.size(2)), i32(kc.size(3)),
-                       i32(kc.size(4)), i32(layer_index), as<int32_t>(block_tables),
+                       head_dim(kc), i32(layer_index), as<int32_t>(block_tables),
                        i32(block_tables.size(1)), as<int32_t>(seq_lens), as<int32_t>(seq_order),
                        i32(query.size(0)), i32(query.size(1)), i32(max_seq_len),
                        static_cast<float>(scale), i32(pages_per_split), out.mutable_data_ptr(),
@@ -185,7 +209,9 @@ void paged_attention_decode(const Tensor &query, const Tensor &key_cache,
         scales);
   };
   const auto none = std::tuple<>();
-  check(k_scales ? call(l.tks_paged_attention_decode_fp8_rows,
+  check(mxfp4(kc) ? call(l.tks_paged_attention_decode_mxfp4,
+                         std::make_tuple(ptr(k_scales), ptr(v_scales)))
+        : k_scales ? call(l.tks_paged_attention_decode_fp8_rows,
                         std::make_tuple(as<const float>(k_scales), as<const float>(v_scales)))
         : fp8(kc) ? call(l.tks_paged_attention_decode_fp8, none, static_cast<float>(k_scale),
                          static_cast<float>(v_scale))
@@ -197,7 +223,7 @@ void paged_attention_decode(const Tensor &query, const Tensor &key_cache,
 Tensor fp8_pages(const Tensor &query, const Tensor &pool, int64_t num_seqs, int64_t table_width,
                  int64_t max_seq_len) {
   return scratch(library().tks_paged_attention_prefill_fp8_workspace_bytes(
-                     i32(num_seqs), i32(query.size(1)), i32(pool.size(2)), i32(pool.size(4)),
+                     i32(num_seqs), i32(query.size(1)), i32(pool.size(2)), head_dim(pool),
                      i32(pool.size(3)), i32(table_width), i32(max_seq_len), code(query)),
                  query, "fp8 prefill");
 }
@@ -209,6 +235,7 @@ void paged_attention_prefill(const Tensor &query, const Tensor &key_cache,
                              int64_t max_query_len, int64_t max_seq_len, double scale,
                              double k_scale, double v_scale, const Tensor &out,
                              const OptTensor &k_scales, const OptTensor &v_scales) {
+  const c10::DeviceGuard guard(query.device());
   const Library &l = library();
   const Tensor &kc = key_cache;
   auto call = [&](auto entry, auto scales, auto... tail) {
@@ -217,7 +244,7 @@ void paged_attention_prefill(const Tensor &query, const Tensor &key_cache,
           return entry(query.const_data_ptr(), query.stride(0), query.stride(1),
                        kc.const_data_ptr(), value_cache.const_data_ptr(), rows...,
                        i32(kc.size(0)), kc.size(1), i32(kc.size(2)), i32(kc.size(3)),
-                       i32(kc.size(4)), i32(layer_index), as<int32_t>(block_tables),
+                       head_dim(kc), i32(layer_index), as<int32_t>(block_tables),
                        i32(block_tables.size(1)), as<int32_t>(seq_lens),
                        as<int32_t>(cu_seqlens_q), as<int32_t>(seq_order), i32(seq_lens.size(0)),
                        query.size(0), i32(query.size(1)), i32(max_query_len), i32(max_seq_len),
@@ -228,7 +255,15 @@ void paged_attention_prefill(const Tensor &query, const Tensor &key_cache,
   };
   const auto none = std::tuple<>();
   int32_t status;
-  if (fp8(kc)) {
+  if (mxfp4(kc)) {
+    const Tensor ws = scratch(l.tks_paged_attention_prefill_mxfp4_workspace_bytes(
+                                  i32(seq_lens.size(0)), i32(kc.size(2)), head_dim(kc),
+                                  i32(kc.size(3)), i32(max_seq_len), code(query)),
+                              query, "MXFP4 prefill");
+    status = call(l.tks_paged_attention_prefill_mxfp4,
+                  std::make_tuple(ptr(k_scales), ptr(v_scales)),
+                  ws.defined() ? ws.mutable_data_ptr() : nullptr, ws.defined() ? ws.numel() : 0);
+  } else if (fp8(kc)) {
     const Tensor ws =
         fp8_pages(query, kc, seq_lens.size(0), block_tables.size(1), max_seq_len);
     void *ws_ptr = ws.defined() ? ws.mutable_data_ptr() : nullptr;
@@ -251,6 +286,7 @@ void rope_append_paged_decode(
     const OptTensor &seq_order, int64_t layer_index, int64_t max_seq_len, double scale,
     int64_t pages_per_split, const Tensor &out, const OptTensor &workspace, double k_scale,
     double v_scale, const OptTensor &k_scales, const OptTensor &v_scales) {
+  const c10::DeviceGuard guard(query.device());
   const Library &l = library();
   const Tensor ws = decode_workspace(workspace, query, key_cache, max_seq_len, pages_per_split);
   void *ws_ptr = ws.defined() ? ws.mutable_data_ptr() : nullptr;
@@ -265,7 +301,7 @@ void rope_append_paged_decode(
                        as<int64_t>(positions), cos.const_data_ptr(), sin.const_data_ptr(),
                        cos.size(0), as<int64_t>(slot_mapping), kc.mutable_data_ptr(),
                        value_cache.mutable_data_ptr(), rows..., i32(kc.size(0)), kc.size(1),
-                       i32(kc.size(2)), i32(kc.size(3)), i32(kc.size(4)), i32(layer_index),
+                       i32(kc.size(2)), i32(kc.size(3)), head_dim(kc), i32(layer_index),
                        as<int32_t>(block_tables), i32(block_tables.size(1)),
                        as<int32_t>(seq_lens), as<int32_t>(seq_order), i32(query.size(0)),
                        i32(query.size(1)), i32(max_seq_len), static_cast<float>(scale),
@@ -276,7 +312,9 @@ void rope_append_paged_decode(
         scales);
   };
   const auto none = std::tuple<>();
-  check(k_scales ? call(l.tks_rope_append_paged_decode_fp8_rows,
+  check(mxfp4(kc) ? call(l.tks_rope_append_paged_decode_mxfp4,
+                         std::make_tuple(mut(k_scales), mut(v_scales)))
+        : k_scales ? call(l.tks_rope_append_paged_decode_fp8_rows,
                         std::make_tuple(as<float>(k_scales), as<float>(v_scales)))
         : fp8(kc) ? call(l.tks_rope_append_paged_decode_fp8, none, static_cast<float>(k_scale),
                          static_cast<float>(v_scale))
@@ -290,6 +328,7 @@ void rope_kv_append(const Tensor &query, const Tensor &key, const Tensor &value,
                     const Tensor &slot_mapping, int64_t layer_index, const Tensor &query_out,
                     const OptTensor &key_out, double k_scale, double v_scale,
                     const OptTensor &k_scales, const OptTensor &v_scales) {
+  const c10::DeviceGuard guard(query.device());
   const Library &l = library();
   const Tensor &kc = key_cache;
   auto call = [&](auto entry, auto scales, auto... factors) {
@@ -301,7 +340,7 @@ void rope_kv_append(const Tensor &query, const Tensor &key, const Tensor &value,
                        key.stride(1), key_out ? key_out->stride(0) : 0,
                        key_out ? key_out->stride(1) : 0, value.const_data_ptr(),
                        value.stride(0), value.stride(1), i32(kc.size(2)), query.size(0),
-                       i32(kc.size(4)), as<int64_t>(positions), cos.const_data_ptr(),
+                       head_dim(kc), as<int64_t>(positions), cos.const_data_ptr(),
                        sin.const_data_ptr(), cos.size(0), kc.mutable_data_ptr(),
                        value_cache.mutable_data_ptr(), rows..., i32(kc.size(0)), kc.size(1),
                        i32(kc.size(3)), i32(layer_index), as<int64_t>(slot_mapping), factors...,
@@ -310,7 +349,9 @@ void rope_kv_append(const Tensor &query, const Tensor &key, const Tensor &value,
         scales);
   };
   const auto none = std::tuple<>();
-  check(k_scales ? call(l.tks_rope_kv_append_fp8_rows,
+  check(mxfp4(kc) ? call(l.tks_rope_kv_append_mxfp4,
+                         std::make_tuple(mut(k_scales), mut(v_scales)))
+        : k_scales ? call(l.tks_rope_kv_append_fp8_rows,
                         std::make_tuple(as<float>(k_scales), as<float>(v_scales)))
         : fp8(kc) ? call(l.tks_rope_kv_append_fp8, none, static_cast<float>(k_scale),
                          static_cast<float>(v_scale))
@@ -326,6 +367,66 @@ void rope_kv_append_(const Tensor &query, const Tensor &key, const Tensor &value
                      const OptTensor &v_scales) {
   rope_kv_append(query, key, value, positions, cos, sin, key_cache, value_cache, slot_mapping,
                  layer_index, query, key_out, k_scale, v_scale, k_scales, v_scales);
+}
+
+void kv_append(const Tensor &key, const Tensor &value, const Tensor &key_cache,
+               const Tensor &value_cache, const Tensor &slot_mapping, int64_t layer_index,
+               double k_scale, double v_scale, const OptTensor &k_scales,
+               const OptTensor &v_scales) {
+  const c10::DeviceGuard guard(key.device());
+  const Library &l = library();
+  const Tensor &kc = key_cache;
+  auto call = [&](auto entry, auto scales, auto... factors) {
+    return std::apply(
+        [&](auto... rows) {
+          return entry(key.const_data_ptr(), key.stride(0), key.stride(1),
+                       value.const_data_ptr(), value.stride(0), value.stride(1), key.size(0),
+                       kc.mutable_data_ptr(), value_cache.mutable_data_ptr(), rows...,
+                       i32(kc.size(0)), kc.size(1), i32(kc.size(2)), i32(kc.size(3)),
+                       head_dim(kc), i32(layer_index), as<int64_t>(slot_mapping), factors...,
+                       code(key), stream_of(key));
+        },
+        scales);
+  };
+  const auto none = std::tuple<>();
+  check(mxfp4(kc) ? call(l.tks_kv_append_mxfp4, std::make_tuple(mut(k_scales), mut(v_scales)))
+        : k_scales ? call(l.tks_kv_append_fp8_rows,
+                          std::make_tuple(as<float>(k_scales), as<float>(v_scales)))
+        : fp8(kc) ? call(l.tks_kv_append_fp8, none, static_cast<float>(k_scale),
+                         static_cast<float>(v_scale))
+                  : call(l.tks_kv_append, none),
+        "kv_append");
+}
+
+void paged_gather(const Tensor &key_cache, const Tensor &value_cache, const Tensor &block_tables,
+                  const Tensor &seq_lens, const Tensor &cu_seqlens, int64_t layer_index,
+                  int64_t max_seq_len, const Tensor &key_out, const Tensor &value_out,
+                  double k_scale, double v_scale, const OptTensor &k_scales,
+                  const OptTensor &v_scales) {
+  const c10::DeviceGuard guard(key_cache.device());
+  const Library &l = library();
+  const Tensor &kc = key_cache;
+  auto call = [&](auto entry, auto scales, auto... factors) {
+    return std::apply(
+        [&](auto... rows) {
+          return entry(kc.const_data_ptr(), value_cache.const_data_ptr(), rows...,
+                       i32(kc.size(0)), kc.size(1), i32(kc.size(2)), i32(kc.size(3)),
+                       head_dim(kc), i32(layer_index), as<int32_t>(block_tables),
+                       i32(block_tables.size(1)), as<int32_t>(seq_lens), as<int32_t>(cu_seqlens),
+                       i32(block_tables.size(0)), i32(max_seq_len), key_out.mutable_data_ptr(),
+                       value_out.mutable_data_ptr(), key_out.stride(0), key_out.stride(1),
+                       factors..., code(key_out), stream_of(key_out));
+        },
+        scales);
+  };
+  const auto none = std::tuple<>();
+  check(mxfp4(kc) ? call(l.tks_paged_gather_mxfp4, std::make_tuple(ptr(k_scales), ptr(v_scales)))
+        : k_scales ? call(l.tks_paged_gather_fp8_rows,
+                          std::make_tuple(as<const float>(k_scales), as<const float>(v_scales)))
+        : fp8(kc) ? call(l.tks_paged_gather_fp8, none, static_cast<float>(k_scale),
+                         static_cast<float>(v_scale))
+                  : call(l.tks_paged_gather, none),
+        "paged_gather");
 }
 
 void rms_norm(const Tensor &input, const Tensor &weight, double epsilon,
@@ -352,6 +453,54 @@ void silu_mul(const Tensor &gate_up, const Tensor &out) {
         "silu_mul");
 }
 
+void mxfp4_quantize(const Tensor &input, const Tensor &codes, const Tensor &scales) {
+  const c10::DeviceGuard guard(input.device());
+  check(library().tks_mxfp4_quantize(input.const_data_ptr(), input.stride(0), input.size(0),
+                                     input.size(1), codes.mutable_data_ptr(),
+                                     scales.mutable_data_ptr(), code(input), stream_of(input)),
+        "mxfp4_quantize");
+}
+
+void mxfp4_dequantize(const Tensor &codes, const Tensor &scales, const Tensor &out) {
+  const c10::DeviceGuard guard(codes.device());
+  check(library().tks_mxfp4_dequantize(codes.const_data_ptr(), scales.const_data_ptr(),
+                                       out.size(0), out.size(1), out.mutable_data_ptr(),
+                                       out.stride(0), code(out), stream_of(out)),
+        "mxfp4_dequantize");
+}
+
+void mxfp4_matmul(const Tensor &a_codes, const Tensor &a_scales, const Tensor &b_codes,
+                  const Tensor &b_scales, const Tensor &out, const OptTensor &workspace) {
+  const c10::DeviceGuard guard(a_codes.device());
+  const Library &l = library();
+  const int64_t m = a_codes.size(0), n = b_codes.size(0), k = 2 * a_codes.size(1);
+  const Tensor ws = workspace ? *workspace
+                              : scratch(l.tks_mxfp4_matmul_workspace_bytes(m, n, k), out,
+                                        "mxfp4_matmul");
+  check(l.tks_mxfp4_matmul(a_codes.const_data_ptr(), a_scales.const_data_ptr(),
+                           b_codes.const_data_ptr(), b_scales.const_data_ptr(), m, n, k,
+                           out.mutable_data_ptr(), out.stride(0),
+                           ws.defined() ? ws.mutable_data_ptr() : nullptr,
+                           ws.defined() ? ws.numel() : 0, code(out), stream_of(out)),
+        "mxfp4_matmul");
+}
+
+void mxfp4_linear(const Tensor &input, const Tensor &weight_codes, const Tensor &weight_scales,
+                  const Tensor &out, const OptTensor &workspace) {
+  const c10::DeviceGuard guard(input.device());
+  const Library &l = library();
+  const int64_t m = input.size(0), n = weight_codes.size(0), k = input.size(1);
+  const Tensor ws = workspace ? *workspace
+                              : scratch(l.tks_mxfp4_linear_workspace_bytes(m, n, k), out,
+                                        "mxfp4_linear");
+  check(l.tks_mxfp4_linear(input.const_data_ptr(), input.stride(0),
+                           weight_codes.const_data_ptr(), weight_scales.const_data_ptr(), m, n, k,
+                           out.mutable_data_ptr(), out.stride(0),
+                           ws.defined() ? ws.mutable_data_ptr() : nullptr,
+                           ws.defined() ? ws.numel() : 0, code(input), stream_of(input)),
+        "mxfp4_linear");
+}
+
 }  // namespace
 
 extern "C" const char *tks_torch_built_for(void) { return TORCH_VERSION; }
@@ -370,9 +519,15 @@ extern "C" const char *tks_torch_register(void) {
       m.impl("rope_append_paged_decode", rope_append_paged_decode);
       m.impl("rope_kv_append", rope_kv_append);
       m.impl("rope_kv_append_", rope_kv_append_);
+      m.impl("kv_append", kv_append);
+      m.impl("paged_gather", paged_gather);
       m.impl("rms_norm", rms_norm);
       m.impl("greedy_argmax", greedy_argmax);
       m.impl("silu_mul", silu_mul);
+      m.impl("mxfp4_quantize", mxfp4_quantize);
+      m.impl("mxfp4_dequantize", mxfp4_dequantize);
+      m.impl("mxfp4_matmul", mxfp4_matmul);
+      m.impl("mxfp4_linear", mxfp4_linear);
       return m;
     }();
   } catch (const std::exception &raised) {

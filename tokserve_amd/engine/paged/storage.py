@@ -15,6 +15,9 @@ row (one token of one KV head) gets a scale of its own, s = max|row| / 448
 (1 for an all-zero or non-finite maximum), kept beside the pools as float32
 [L, NB, Hkv, BS] arrays that the append kernels write and the attention and
 gather kernels read (4 bytes per Dh code bytes: 1/32 more at Dh 128).
+`kv_dtype=torch.float4_e2m1fn_x2` stores K and V in MXFP4 (17 bytes for 32 values of a
+row: e2m1 codes, [L, NB, Hkv, BS, Dh / 2], and one e8m0 scale per 32, [L, NB, Hkv, BS,
+Dh / 32]; head_dim 32, 64, 96 or 128), 17/64 of the bytes of bf16 pools.
 """
 
 from __future__ import annotations
@@ -61,8 +64,12 @@ class PagedKVStorage:
         self.device = torch.device(device)
         self.dtype = dtype
         self.kv_dtype = dtype if kv_dtype is None else kv_dtype
-        if self.kv_dtype not in (dtype, ops.FP8_POOL_DTYPE):
-            raise ValueError("kv_dtype must be the model dtype or torch.float8_e4m3fn")
+        if self.kv_dtype not in (dtype, ops.FP8_POOL_DTYPE, ops.MXFP4_DTYPE):
+            raise ValueError("kv_dtype must be the model dtype or torch.float8_e4m3fn "
+                             "or torch.float4_e2m1fn_x2")
+        mxfp4 = self.kv_dtype == ops.MXFP4_DTYPE
+        if mxfp4 and head_dim not in ops.MXFP4_HEAD_DIMS:
+            raise ValueError("MXFP4 pools need a head_dim of 32, 64, 96 or 128")
         self.k_scale = float(k_scale)
         self.v_scale = float(v_scale)
         if self.kv_dtype == ops.FP8_POOL_DTYPE:
@@ -76,7 +83,8 @@ class PagedKVStorage:
                                            or self.k_scale != 1.0 or self.v_scale != 1.0):
             raise ValueError("per-row scales need fp8 pools and no pool scales")
         self.scale_granularity = scale_granularity
-        shape = (num_layers, num_blocks, num_key_value_heads, block_size, head_dim)
+        shape = (num_layers, num_blocks, num_key_value_heads, block_size,
+                 head_dim // 2 if mxfp4 else head_dim)
         self._key_storage = torch.empty(shape, device=self.device, dtype=self.kv_dtype)
         self._value_storage = torch.empty(shape, device=self.device, dtype=self.kv_dtype)
         self._key_scales: torch.Tensor | None = None
@@ -84,6 +92,11 @@ class PagedKVStorage:
         if scale_granularity == "row":
             self._key_scales = torch.ones(shape[:4], device=self.device, dtype=torch.float32)
             self._value_scales = torch.ones(shape[:4], device=self.device, dtype=torch.float32)
+        elif mxfp4:
+            blocks = (*shape[:4], head_dim // ops.MXFP4_BLOCK)
+            self._key_scales = torch.empty(blocks, device=self.device, dtype=ops.MXFP4_SCALE_DTYPE)
+            self._value_scales = torch.empty(blocks, device=self.device,
+                                             dtype=ops.MXFP4_SCALE_DTYPE)
 
     @property
     def storage_shape(self) -> tuple[int, ...]:
@@ -103,20 +116,22 @@ class PagedKVStorage:
 
     @property
     def key_scales(self) -> torch.Tensor | None:
-        """Per-row K scales, float32 [L, NB, Hkv, BS] (None with per-pool scales)."""
+        """Per-row K scales, float32 [L, NB, Hkv, BS], or those of MXFP4 blocks (None with
+        per-pool scales)."""
 
         return self._key_scales
 
     @property
     def value_scales(self) -> torch.Tensor | None:
-        """Per-row V scales, float32 [L, NB, Hkv, BS] (None with per-pool scales)."""
+        """Per-row V scales, float32 [L, NB, Hkv, BS], or those of MXFP4 blocks (None with
+        per-pool scales)."""
 
         return self._value_scales
 
     @property
     def scales(self) -> dict[str, float | torch.Tensor]:
         """Decode factors as the kernels' keyword arguments: the pool scales, or the
-        per-row scale arrays."""
+        per-row or per-block scale arrays."""
 
         if self._key_scales is not None:
             return {"k_scales": self._key_scales, "v_scales": self._value_scales}

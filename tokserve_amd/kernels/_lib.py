@@ -15,7 +15,7 @@ from pathlib import Path
 import torch
 
 LIBRARY_NAME = "libtokserve_hip.so"
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 TKS_OK = 0
 TKS_ERR_VALUE = -1
@@ -181,6 +181,74 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _i64, _i32, _i32, _i32, _i32,
          _c_void_p, _i32, _c_void_p, _c_void_p, _i32, _i32, _i32, _f32, _i32,
          _c_void_p, _i64, _i64, _c_void_p, _i64, _i32, _c_void_p],
+    ),
+    # MXFP4: products, and pools whose scale bytes follow them.
+    "tks_mxfp4_quantize": (
+        _i32,
+        [_c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _i32, _c_void_p],
+    ),
+    "tks_mxfp4_dequantize": (
+        _i32,
+        [_c_void_p, _c_void_p, _i64, _i64, _c_void_p, _i64, _i32, _c_void_p],
+    ),
+    "tks_mxfp4_matmul_workspace_bytes": (
+        _i64,
+        [_i64, _i64, _i64],
+    ),
+    "tks_mxfp4_matmul": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _c_void_p, _i64,
+         _c_void_p, _i64, _i32, _c_void_p],
+    ),
+    "tks_mxfp4_linear_workspace_bytes": (
+        _i64,
+        [_i64, _i64, _i64],
+    ),
+    "tks_mxfp4_linear": (
+        _i32,
+        [_c_void_p, _i64, _c_void_p, _c_void_p, _i64, _i64, _i64, _c_void_p, _i64, _c_void_p,
+         _i64, _i32, _c_void_p],
+    ),
+    "tks_kv_append_mxfp4": (
+        _i32,
+        [_c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _c_void_p,
+         _c_void_p, _i32, _i64, _i32, _i32, _i32, _i32, _c_void_p, _i32, _c_void_p],
+    ),
+    "tks_paged_gather_mxfp4": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _i64, _i32, _i32, _i32, _i32,
+         _c_void_p, _i32, _c_void_p, _c_void_p, _i32, _i32, _c_void_p, _c_void_p, _i64, _i64,
+         _i32, _c_void_p],
+    ),
+    "tks_rope_kv_append_mxfp4": (
+        _i32,
+        [_c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i32, _c_void_p, _c_void_p, _i64, _i64,
+         _i64, _i64, _c_void_p, _i64, _i64, _i32, _i64, _i32, _c_void_p, _c_void_p, _c_void_p,
+         _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _i64, _i32, _i32, _c_void_p,
+         _i32, _c_void_p],
+    ),
+    "tks_paged_attention_decode_mxfp4": (
+        _i32,
+        [_c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _i64, _i32,
+         _i32, _i32, _i32, _c_void_p, _i32, _c_void_p, _c_void_p, _i32, _i32, _i32, _f32, _i32,
+         _c_void_p, _i64, _i64, _c_void_p, _i64, _i32, _c_void_p],
+    ),
+    "tks_rope_append_paged_decode_mxfp4": (
+        _i32,
+        [_c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p,
+         _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32,
+         _i64, _i32, _i32, _i32, _i32, _c_void_p, _i32, _c_void_p, _c_void_p, _i32, _i32, _i32,
+         _f32, _i32, _c_void_p, _i64, _i64, _c_void_p, _i64, _i32, _c_void_p],
+    ),
+    "tks_paged_attention_prefill_mxfp4_workspace_bytes": (
+        _i64,
+        [_i32, _i32, _i32, _i32, _i32, _i32],
+    ),
+    "tks_paged_attention_prefill_mxfp4": (
+        _i32,
+        [_c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _i64, _i32,
+         _i32, _i32, _i32, _c_void_p, _i32, _c_void_p, _c_void_p, _c_void_p, _i32, _i64, _i32,
+         _i32, _i32, _f32, _c_void_p, _i64, _i64, _c_void_p, _i64, _i32, _c_void_p],
     ),
 }
 

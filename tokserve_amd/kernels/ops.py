@@ -40,6 +40,11 @@ def _pool_shape(key_cache: torch.Tensor, value_cache: torch.Tensor) -> tuple[int
         raise ValueError("KV pools must use the same dtype")
     if not key_cache.is_contiguous() or not value_cache.is_contiguous():
         raise ValueError("KV pools must be contiguous")
+    if is_mxfp4_pool(key_cache):
+        head_dim = 2 * key_cache.shape[4]
+        if head_dim not in MXFP4_HEAD_DIMS:
+            raise ValueError("MXFP4 KV pools need a head_dim of 32, 64, 96 or 128")
+        return (*key_cache.shape[:4], head_dim)
     return tuple(key_cache.shape)
 
 
@@ -51,6 +56,29 @@ FP8_POOL_DTYPE = torch.float8_e4m3fn
 
 def is_fp8_pool(pool: torch.Tensor) -> bool:
     return pool.dtype == FP8_POOL_DTYPE
+
+
+# MXFP4: 32 consecutive values x share one power-of-two scale s (an e8m0 byte) and are held
+# as e2m1 codes, two to an element of MXFP4_DTYPE (the even value in the low nibble):
+#   s = 2^(floor(log2(max|x|)) - 2), between 2^-125 and 2^125;
+#   code = x / s rounded to nearest among 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives,
+#   ties to the even code, at most 6 in magnitude; decoded = code * s.
+# A block with a NaN or an infinity has the scale NaN and reads back as NaN. Matrices are
+# codes (rows, cols / 2) and scales (rows, cols / 32); K/V pools codes
+# (L, NB, Hkv, BS, Dh / 2) and scales (L, NB, Hkv, BS, Dh / 32), given as k_scales and
+# v_scales wherever the fp8 pools' row scales are.
+MXFP4_DTYPE = torch_ops.MXFP4_POOL_DTYPE
+MXFP4_SCALE_DTYPE = torch.float8_e8m0fnu
+MXFP4_BLOCK = 32
+MXFP4_HEAD_DIMS = (32, 64, 96, 128)
+
+
+def is_mxfp4_pool(pool: torch.Tensor) -> bool:
+    return pool.dtype == MXFP4_DTYPE
+
+
+def _is_quantized_pool(pool: torch.Tensor) -> bool:
+    return is_fp8_pool(pool) or is_mxfp4_pool(pool)
 
 
 def _pool_scales(pool: torch.Tensor, k_scale: float, v_scale: float) -> tuple[float, float]:
@@ -78,13 +106,26 @@ def _row_scales(
 
     Row (l, b, h, r) of a pool holds e4m3(clamp(x / s, -448, 448)) with
     s = k_scales[l, b, h, r] (v_scales for the value pool), decoded as code * s;
-    the pool scales must then stay 1.
+    the pool scales must then stay 1. MXFP4 pools always have theirs, float8_e8m0fnu
+    (L, NB, Hkv, BS, Dh / 32).
     """
 
+    mxfp4 = is_mxfp4_pool(key_cache)
     if k_scales is None and v_scales is None:
+        if mxfp4:
+            raise ValueError(f"{operation}: MXFP4 KV pools need k_scales and v_scales")
         return None, None
     if k_scales is None or v_scales is None:
         raise ValueError(f"{operation}: k_scales and v_scales go together")
+    if mxfp4:
+        require_hip(operation, key_cache, k_scales, v_scales)
+        shape = (*key_cache.shape[:4], 2 * key_cache.shape[4] // MXFP4_BLOCK)
+        for name, scales in (("k_scales", k_scales), ("v_scales", v_scales)):
+            if scales.dtype != MXFP4_SCALE_DTYPE:
+                raise TypeError(f"{name} of MXFP4 pools must be float8_e8m0fnu")
+            if scales.shape != shape or not scales.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous (L, NB, Hkv, BS, Dh / 32) tensor")
+        return k_scales, v_scales
     if not is_fp8_pool(key_cache):
         raise ValueError("per-row scales apply to fp8 KV pools only")
     if k_scale != 1.0 or v_scale != 1.0:
@@ -130,7 +171,8 @@ def kv_append(
     fp8 pools quantize the rows with the pool scales (k_scale, v_scale), or, given
     k_scales / v_scales (float32 (L, NB, Hkv, BS)), each row with a scale of its
     own, s = max|row| / 448 (1 for an all-zero or non-finite maximum), written to
-    the row's entry of k_scales / v_scales. Pools in a float dtype take rows of
+    the row's entry of k_scales / v_scales. MXFP4 pools quantize each block of 32 with
+    its scale, written to k_scales / v_scales. Pools in a float dtype take rows of
     that dtype, copied bit for bit.
     """
 
@@ -142,10 +184,10 @@ def kv_append(
         raise ValueError("key and value must have shape (N, Hkv, Dh)")
     if key.shape[1:] != (num_kv_heads, head_dim):
         raise ValueError("key rows must match the pool's (Hkv, Dh)")
-    fp8 = is_fp8_pool(key_cache)
+    quantized = _is_quantized_pool(key_cache)
     k_scale, v_scale = _pool_scales(key_cache, k_scale, v_scale)
     k_scales, v_scales = _row_scales("kv_append", key_cache, k_scales, v_scales, k_scale, v_scale)
-    if value.dtype != key.dtype or (not fp8 and key.dtype != key_cache.dtype):
+    if value.dtype != key.dtype or (not quantized and key.dtype != key_cache.dtype):
         raise ValueError("keys and values must match the storage dtype")
     if slot_mapping.shape != (key.shape[0],):
         raise ValueError("slot_mapping must have shape (N,)")
@@ -176,7 +218,7 @@ def paged_gather(
 
     key_out/value_out are (S_total, Hkv, Dh) views (any token/head strides, Dh
     contiguous); sequence b fills rows cu_seqlens[b] .. cu_seqlens[b]+seq_lens[b]-1.
-    fp8 pools are decoded with their scales (per pool, or per row with
+    fp8 and MXFP4 pools are decoded with their scales (per pool, or those of
     k_scales / v_scales) into the outputs' float dtype.
     """
 
@@ -198,11 +240,11 @@ def paged_gather(
         raise ValueError("key_out and value_out must share shape and strides")
     if key_out.stride(-1) != 1:
         raise ValueError("outputs must be contiguous in head_dim")
-    fp8 = is_fp8_pool(key_cache)
+    quantized = _is_quantized_pool(key_cache)
     k_scale, v_scale = _pool_scales(key_cache, k_scale, v_scale)
     k_scales, v_scales = _row_scales("paged_gather", key_cache, k_scales, v_scales, k_scale,
                                      v_scale)
-    if value_out.dtype != key_out.dtype or (not fp8 and key_out.dtype != key_cache.dtype):
+    if value_out.dtype != key_out.dtype or (not quantized and key_out.dtype != key_cache.dtype):
         raise ValueError("outputs must match the storage dtype")
     _ops.paged_gather(key_cache, value_cache, tables, lens, cu, layer_index, max_seq_len,
                       key_out, value_out, k_scale, v_scale, k_scales, v_scales)
@@ -292,7 +334,8 @@ def paged_attention_decode(
     `seq_order` (int32 permutation of 0..B-1, see longest_first) is the order in
     which sequences reach workgroups; longest-first avoids a tail of long
     sequences. Results do not depend on it. fp8 pools are decoded with
-    (k_scale, v_scale), or per row with k_scales / v_scales.
+    (k_scale, v_scale), or per row with k_scales / v_scales, MXFP4 pools with
+    k_scales / v_scales (their values exact whatever the query's dtype).
     """
 
     require_hip("paged_attention_decode", query, key_cache, value_cache, block_tables, seq_lens)
@@ -301,11 +344,11 @@ def paged_attention_decode(
     )
     if query.ndim != 3 or query.shape[2] != head_dim:
         raise ValueError("query must have shape (B, Hq, Dh) with the pool's Dh")
-    fp8 = is_fp8_pool(key_cache)
+    quantized = _is_quantized_pool(key_cache)
     k_scale, v_scale = _pool_scales(key_cache, k_scale, v_scale)
     k_scales, v_scales = _row_scales("paged_attention_decode", key_cache, k_scales, v_scales,
                                      k_scale, v_scale)
-    if not fp8 and query.dtype != key_cache.dtype:
+    if not quantized and query.dtype != key_cache.dtype:
         raise ValueError("query and paged storage must use the same dtype")
     num_seqs, num_q_heads, _ = query.shape
     if num_q_heads % num_kv_heads != 0:
@@ -394,7 +437,8 @@ def paged_attention_prefill(
     position seq_lens[b] - q_len_b + i. `seq_order` (int32 permutation of 0..B-1,
     e.g. longest_first of seq_lens) is the order in which sequences reach
     workgroups; results do not depend on it. fp8 pools are decoded with
-    (k_scale, v_scale), or per row with k_scales / v_scales.
+    (k_scale, v_scale), or per row with k_scales / v_scales; MXFP4 pools with
+    k_scales / v_scales, their values rounded to the query's dtype.
     """
 
     require_hip(
@@ -406,11 +450,11 @@ def paged_attention_prefill(
     )
     if query.ndim != 3 or query.shape[2] != head_dim:
         raise ValueError("query must have shape (N, Hq, Dh) with the pool's Dh")
-    fp8 = is_fp8_pool(key_cache)
+    quantized = _is_quantized_pool(key_cache)
     k_scale, v_scale = _pool_scales(key_cache, k_scale, v_scale)
     k_scales, v_scales = _row_scales("paged_attention_prefill", key_cache, k_scales, v_scales,
                                      k_scale, v_scale)
-    if not fp8 and query.dtype != key_cache.dtype:
+    if not quantized and query.dtype != key_cache.dtype:
         raise ValueError("query and paged storage must use the same dtype")
     num_q_heads = query.shape[1]
     if num_q_heads % num_kv_heads != 0:
@@ -431,6 +475,176 @@ def paged_attention_prefill(
                                  layer_index, max_query_len, max_seq_len, float(scale), k_scale,
                                  v_scale, out, k_scales, v_scales)
     return out
+
+
+# ----------------------------------------------------------------------------
+# MXFP4 matrices
+
+
+def _float_rows(operation: str, tensor: torch.Tensor, name: str) -> torch.Tensor:
+    """(..., K) float values as rows (R, K), K contiguous and whole MXFP4 blocks."""
+
+    if tensor.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise TypeError(f"{operation}: {name} must be float32, float16 or bfloat16")
+    if tensor.ndim < 1 or tensor.shape[-1] < 1 or tensor.shape[-1] % MXFP4_BLOCK != 0:
+        raise ValueError(f"{operation}: the last dimension of {name} must be a positive multiple "
+                         "of 32")
+    # (numel is 0 without rows, where -1 could not be inferred)
+    rows = tensor.reshape(tensor.numel() // tensor.shape[-1], tensor.shape[-1])
+    return _last_dim_contiguous(rows, name)
+
+
+def _mxfp4_operand(operation: str, codes: torch.Tensor, scales: torch.Tensor, name: str) -> int:
+    """Checks one MXFP4 tensor, codes (..., K / 2) and scales (..., K / 32); returns K."""
+
+    require_hip(operation, codes, scales)
+    if codes.dtype != MXFP4_DTYPE or scales.dtype != MXFP4_SCALE_DTYPE:
+        raise TypeError(f"{operation}: {name} codes must be float4_e2m1fn_x2 and scales "
+                        "float8_e8m0fnu")
+    depth = 2 * codes.shape[-1] if codes.ndim else 0
+    if depth < 1 or depth % MXFP4_BLOCK != 0:
+        raise ValueError(f"{operation}: {name} must hold a positive multiple of 32 values a row")
+    if scales.shape != (*codes.shape[:-1], depth // MXFP4_BLOCK):
+        raise ValueError(f"{operation}: {name} scales must have one entry per 32 values")
+    if not codes.is_contiguous() or not scales.is_contiguous():
+        raise ValueError(f"{operation}: {name} codes and scales must be contiguous")
+    return depth
+
+
+def _product_out(operation: str, like: torch.Tensor, shape: tuple[int, ...], dtype: torch.dtype,
+                 out: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The output (given or new) and its rows."""
+
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=like.device)
+    require_hip(operation, like, out)
+    if out.shape != shape or out.dtype != dtype or (out.numel() and out.stride(-1) != 1):
+        raise ValueError(f"{operation}: out must have shape {tuple(shape)} and the dtype {dtype}, "
+                         "its last dimension contiguous")
+    if out.ndim == 2:
+        return out, out
+    if not out.is_contiguous():
+        raise ValueError(f"{operation}: an out of more than two dimensions must be contiguous")
+    return out, out.view(out.numel() // shape[-1], shape[-1])
+
+
+def mxfp4_quantize(
+    inputs: torch.Tensor,
+    *,
+    codes: torch.Tensor | None = None,
+    scales: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """(..., K) values to MXFP4: codes (..., K / 2) float4_e2m1fn_x2 and scales (..., K / 32)
+    float8_e8m0fnu, blocks of 32 along the last dimension (K a multiple of 32)."""
+
+    require_hip("mxfp4_quantize", inputs)
+    rows = _float_rows("mxfp4_quantize", inputs, "inputs")
+    lead, depth = inputs.shape[:-1], inputs.shape[-1]
+    if codes is None:
+        codes = torch.empty((*lead, depth // 2), dtype=MXFP4_DTYPE, device=inputs.device)
+    if scales is None:
+        scales = torch.empty((*lead, depth // MXFP4_BLOCK), dtype=MXFP4_SCALE_DTYPE,
+                             device=inputs.device)
+    require_hip("mxfp4_quantize", inputs, codes)
+    if codes.shape != (*lead, depth // 2):
+        raise ValueError("mxfp4_quantize: codes must have shape (..., K / 2)")
+    _mxfp4_operand("mxfp4_quantize", codes, scales, "output")
+    _ops.mxfp4_quantize(rows, codes, scales)
+    return codes, scales
+
+
+def mxfp4_dequantize(
+    codes: torch.Tensor,
+    scales: torch.Tensor,
+    dtype: torch.dtype,
+    *,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """The values (..., K) of codes (..., K / 2) and scales (..., K / 32), rounded to dtype
+    (exact in float32 and bfloat16)."""
+
+    depth = _mxfp4_operand("mxfp4_dequantize", codes, scales, "input")
+    if dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise TypeError("mxfp4_dequantize: dtype must be float32, float16 or bfloat16")
+    out, rows = _product_out("mxfp4_dequantize", codes, (*codes.shape[:-1], depth), dtype, out)
+    _ops.mxfp4_dequantize(codes, scales, rows)
+    return out
+
+
+def mxfp4_matmul(
+    a_codes: torch.Tensor,
+    a_scales: torch.Tensor,
+    b_codes: torch.Tensor,
+    b_scales: torch.Tensor,
+    dtype: torch.dtype,
+    *,
+    out: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """A B^T of MXFP4 matrices A (..., M, K) and B (N, K), each as its codes and scales, summed
+    in fp32 and rounded once to dtype: (..., M, N).
+
+    `workspace` (uint8, of mxfp4_matmul_workspace_bytes) is scratch memory; calls that share
+    one must be ordered on one stream. It is allocated when it is not given.
+    """
+
+    depth = _mxfp4_operand("mxfp4_matmul", a_codes, a_scales, "A")
+    if b_codes.ndim != 2 or _mxfp4_operand("mxfp4_matmul", b_codes, b_scales, "B") != depth:
+        raise ValueError("mxfp4_matmul: B must have shape (N, K) with A's K")
+    require_hip("mxfp4_matmul", a_codes, b_codes)
+    if b_codes.shape[0] < 1:
+        raise ValueError("mxfp4_matmul: B must have at least one row")
+    if dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise TypeError("mxfp4_matmul: dtype must be float32, float16 or bfloat16")
+    out, rows = _product_out("mxfp4_matmul", a_codes, (*a_codes.shape[:-1], b_codes.shape[0]),
+                             dtype, out)
+    _check_workspace("mxfp4_matmul", a_codes, workspace)
+    _ops.mxfp4_matmul(a_codes.view(rows.shape[0], depth // 2), a_scales,
+                      b_codes, b_scales, rows, workspace)
+    return out
+
+
+def mxfp4_linear(
+    inputs: torch.Tensor,
+    weight_codes: torch.Tensor,
+    weight_scales: torch.Tensor,
+    *,
+    out: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """A projection with MXFP4 weights (N, K): inputs (..., K) -> (..., N) in their dtype.
+
+    The rows are quantized as mxfp4_quantize does and multiplied as mxfp4_matmul does; the
+    results are those of the two calls. `workspace` as there, of mxfp4_linear_workspace_bytes.
+    """
+
+    require_hip("mxfp4_linear", inputs, weight_codes)
+    rows_in = _float_rows("mxfp4_linear", inputs, "inputs")
+    if (weight_codes.ndim != 2
+            or _mxfp4_operand("mxfp4_linear", weight_codes, weight_scales, "weight")
+            != inputs.shape[-1]):
+        raise ValueError("mxfp4_linear: the weight must have shape (N, K) with the inputs' K")
+    if weight_codes.shape[0] < 1:
+        raise ValueError("mxfp4_linear: the weight must have at least one row")
+    out, rows = _product_out("mxfp4_linear", inputs, (*inputs.shape[:-1], weight_codes.shape[0]),
+                             inputs.dtype, out)
+    _check_workspace("mxfp4_linear", inputs, workspace)
+    _ops.mxfp4_linear(rows_in, weight_codes, weight_scales, rows, workspace)
+    return out
+
+
+def mxfp4_matmul_workspace_bytes(num_rows: int, num_cols: int, depth: int) -> int:
+    """Bytes of scratch mxfp4_matmul needs for (M, K) x (N, K)."""
+
+    return torch_ops.product_workspace_bytes("tks_mxfp4_matmul_workspace_bytes", num_rows,
+                                             num_cols, depth)
+
+
+def mxfp4_linear_workspace_bytes(num_rows: int, num_cols: int, depth: int) -> int:
+    """Bytes of scratch mxfp4_linear needs for M rows of K values and weights (N, K)."""
+
+    return torch_ops.product_workspace_bytes("tks_mxfp4_linear_workspace_bytes", num_rows,
+                                             num_cols, depth)
 
 
 # ----------------------------------------------------------------------------
@@ -599,8 +813,8 @@ def rope_kv_append(
 
     One launch, bit-identical to rope() followed by kv_append() of the rotated keys.
     key_out, when given, also receives the rotated keys. Pools in the rows' dtype, or
-    fp8 pools quantized with k_scale / v_scale, or per row into k_scales / v_scales, as
-    kv_append() does.
+    fp8 pools quantized with k_scale / v_scale, or per row into k_scales / v_scales, or
+    MXFP4 pools, as kv_append() does.
     """
 
     require_hip("rope_kv_append", query, key, value, positions, key_cache, value_cache,
@@ -616,7 +830,7 @@ def rope_kv_append(
     k_scale, v_scale = _pool_scales(key_cache, k_scale, v_scale)
     k_scales, v_scales = _row_scales("rope_kv_append", key_cache, k_scales, v_scales, k_scale,
                                      v_scale)
-    pool_dtype = query.dtype if is_fp8_pool(key_cache) else key_cache.dtype
+    pool_dtype = query.dtype if _is_quantized_pool(key_cache) else key_cache.dtype
     if len({query.dtype, key.dtype, value.dtype, pool_dtype, table.dtype}) != 1:
         raise ValueError("query, key, value, pools and the rotary table must share a dtype")
     if head_dim != table.head_dim:
@@ -678,7 +892,8 @@ def rope_append_paged_decode(
     Bit-identical to rope_kv_append() followed by paged_attention_decode() with the
     same arguments (one launch on the MFMA decode kernel; with per-row scales the append
     is a launch of its own ahead of the attention). Pools in the rows' dtype, or fp8
-    pools with their scales (per pool, or per row with k_scales / v_scales).
+    pools with their scales (per pool, or per row with k_scales / v_scales), or MXFP4
+    pools with theirs (the append a launch of its own).
     """
 
     require_hip("rope_append_paged_decode", query, key, value, positions, key_cache,
@@ -694,7 +909,7 @@ def rope_append_paged_decode(
     num_seqs, num_q_heads, _ = query.shape
     if key.shape != (num_seqs, num_kv_heads, head_dim) or query.shape[2] != head_dim:
         raise ValueError("key and value rows must match the pool's (Hkv, Dh)")
-    pool_dtype = query.dtype if is_fp8_pool(key_cache) else key_cache.dtype
+    pool_dtype = query.dtype if _is_quantized_pool(key_cache) else key_cache.dtype
     if len({query.dtype, key.dtype, value.dtype, pool_dtype, table.dtype}) != 1:
         raise ValueError("query, key, value, pools and the rotary table must share a dtype")
     if head_dim != table.head_dim:

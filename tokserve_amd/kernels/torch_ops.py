@@ -47,6 +47,7 @@ from tokserve_amd.kernels import _lib
 NAMESPACE = "tokserve_amd"
 
 FP8_POOL_DTYPE = torch.float8_e4m3fn
+MXFP4_POOL_DTYPE = torch.float4_e2m1fn_x2  # two codes to an element
 
 SCHEMAS = {
     "kv_append": (
@@ -115,34 +116,64 @@ SCHEMAS = {
     "vector_add": "vector_add(Tensor x, Tensor y, Tensor(a!) out) -> ()",
 }
 
+# Operators on MXFP4 matrices: codes (rows, cols / 2) float4_e2m1fn_x2, scales
+# (rows, cols / 32) float8_e8m0fnu.
+MXFP4_SCHEMAS = {
+    "mxfp4_quantize": (
+        "mxfp4_quantize(Tensor input, Tensor(a!) codes, Tensor(b!) scales) -> ()"
+    ),
+    "mxfp4_dequantize": (
+        "mxfp4_dequantize(Tensor codes, Tensor scales, Tensor(a!) out) -> ()"
+    ),
+    "mxfp4_matmul": (
+        "mxfp4_matmul(Tensor a_codes, Tensor a_scales, Tensor b_codes, Tensor b_scales, "
+        "Tensor(a!) out, Tensor(b!)? workspace=None) -> ()"
+    ),
+    "mxfp4_linear": (
+        "mxfp4_linear(Tensor input, Tensor weight_codes, Tensor weight_scales, Tensor(a!) out, "
+        "Tensor(b!)? workspace=None) -> ()"
+    ),
+}
+
 # Entry points behind each operator (the *_fp8 ones serve e4m3 pools with one scale per
-# pool, the *_fp8_rows ones e4m3 pools with one scale per pool row).
+# pool, the *_fp8_rows ones e4m3 pools with one scale per pool row, the *_mxfp4 ones MXFP4
+# pools).
 ENTRY_POINTS = {
-    "kv_append": ("tks_kv_append", "tks_kv_append_fp8", "tks_kv_append_fp8_rows"),
-    "paged_gather": ("tks_paged_gather", "tks_paged_gather_fp8", "tks_paged_gather_fp8_rows"),
+    "kv_append": ("tks_kv_append", "tks_kv_append_fp8", "tks_kv_append_fp8_rows",
+                  "tks_kv_append_mxfp4"),
+    "paged_gather": ("tks_paged_gather", "tks_paged_gather_fp8", "tks_paged_gather_fp8_rows",
+                     "tks_paged_gather_mxfp4"),
     "paged_attention_decode": ("tks_paged_attention_decode_workspace_bytes",
                                "tks_paged_attention_decode", "tks_paged_attention_decode_fp8",
-                               "tks_paged_attention_decode_fp8_rows"),
+                               "tks_paged_attention_decode_fp8_rows",
+                               "tks_paged_attention_decode_mxfp4"),
     "paged_attention_decode_noalloc": ("tks_paged_attention_decode_noalloc",
                                        "tks_paged_attention_decode_noalloc_max_workspace_bytes"),
     "paged_attention_prefill": ("tks_paged_attention_prefill",
                                 "tks_paged_attention_prefill_fp8_workspace_bytes",
                                 "tks_paged_attention_prefill_fp8",
-                                "tks_paged_attention_prefill_fp8_rows"),
+                                "tks_paged_attention_prefill_fp8_rows",
+                                "tks_paged_attention_prefill_mxfp4_workspace_bytes",
+                                "tks_paged_attention_prefill_mxfp4"),
     "rms_norm": ("tks_rms_norm",),
     "rope": ("tks_rope",),
     "rope_": ("tks_rope",),
     "rope_kv_append": ("tks_rope_kv_append", "tks_rope_kv_append_fp8",
-                       "tks_rope_kv_append_fp8_rows"),
+                       "tks_rope_kv_append_fp8_rows", "tks_rope_kv_append_mxfp4"),
     "rope_kv_append_": ("tks_rope_kv_append", "tks_rope_kv_append_fp8",
-                        "tks_rope_kv_append_fp8_rows"),
+                        "tks_rope_kv_append_fp8_rows", "tks_rope_kv_append_mxfp4"),
     "rope_append_paged_decode": ("tks_rope_append_paged_decode",
                                  "tks_rope_append_paged_decode_fp8",
                                  "tks_rope_append_paged_decode_fp8_rows",
+                                 "tks_rope_append_paged_decode_mxfp4",
                                  "tks_paged_attention_decode_workspace_bytes"),
     "greedy_argmax": ("tks_argmax",),
     "silu_mul": ("tks_silu_mul",),
     "vector_add": ("tks_vector_add",),
+    "mxfp4_quantize": ("tks_mxfp4_quantize",),
+    "mxfp4_dequantize": ("tks_mxfp4_dequantize",),
+    "mxfp4_matmul": ("tks_mxfp4_matmul", "tks_mxfp4_matmul_workspace_bytes"),
+    "mxfp4_linear": ("tks_mxfp4_linear", "tks_mxfp4_linear_workspace_bytes"),
 }
 
 
@@ -192,48 +223,17 @@ def decode_workspace_bytes(num_seqs: int, num_q_heads: int, num_kv_heads: int, h
     return int(size)
 
 
+def product_workspace_bytes(query: str, num_rows: int, num_cols: int, depth: int) -> int:
+    """The answer of an MXFP4 product's size query."""
+
+    size = getattr(_lib.load(), query)(num_rows, num_cols, depth)
+    if size < 0:
+        raise ValueError("invalid MXFP4 product workspace query")
+    return int(size)
+
+
 # ----------------------------------------------------------------------------
 # Device kernels
-
-
-def _kv_append(key, value, key_cache, value_cache, slot_mapping, layer_index, k_scale, v_scale,
-               k_scales=None, v_scales=None):
-    dims = _pool_dims(key_cache)
-    rows = (key.data_ptr(), key.stride(0), key.stride(1),
-            value.data_ptr(), value.stride(0), value.stride(1), key.shape[0],
-            key_cache.data_ptr(), value_cache.data_ptr())
-    common = (*rows, *dims, layer_index, slot_mapping.data_ptr())
-    library = _lib.load()
-    if k_scales is not None:
-        status = library.tks_kv_append_fp8_rows(*rows, k_scales.data_ptr(), v_scales.data_ptr(),
-                                                *dims, layer_index, slot_mapping.data_ptr(),
-                                                _code(key), _stream(key))
-    elif key_cache.dtype == FP8_POOL_DTYPE:
-        status = library.tks_kv_append_fp8(*common, k_scale, v_scale, _code(key), _stream(key))
-    else:
-        status = library.tks_kv_append(*common, _code(key), _stream(key))
-    _lib.check(status, "kv_append")
-
-
-def _paged_gather(key_cache, value_cache, block_tables, seq_lens, cu_seqlens, layer_index,
-                  max_seq_len, key_out, value_out, k_scale, v_scale, k_scales=None,
-                  v_scales=None):
-    rest = (*_pool_dims(key_cache), layer_index,
-            block_tables.data_ptr(), block_tables.shape[1], seq_lens.data_ptr(),
-            cu_seqlens.data_ptr(), block_tables.shape[0], max_seq_len,
-            key_out.data_ptr(), value_out.data_ptr(), key_out.stride(0), key_out.stride(1))
-    common = (key_cache.data_ptr(), value_cache.data_ptr(), *rest)
-    library = _lib.load()
-    if k_scales is not None:
-        status = library.tks_paged_gather_fp8_rows(
-            key_cache.data_ptr(), value_cache.data_ptr(), k_scales.data_ptr(),
-            v_scales.data_ptr(), *rest, _code(key_out), _stream(key_cache))
-    elif key_cache.dtype == FP8_POOL_DTYPE:
-        status = library.tks_paged_gather_fp8(*common, k_scale, v_scale, _code(key_out),
-                                              _stream(key_cache))
-    else:
-        status = library.tks_paged_gather(*common, _code(key_out), _stream(key_cache))
-    _lib.check(status, "paged_gather")
 
 
 def _decode_common(query, key_cache, value_cache, block_tables, seq_lens, seq_order,
@@ -284,8 +284,6 @@ def _vector_add(x, y, out):
 
 # Operators with a device kernel here; the others' are native (csrc/torch_ops.cpp).
 KERNELS = {
-    "kv_append": _kv_append,
-    "paged_gather": _paged_gather,
     "paged_attention_decode_noalloc": _paged_attention_decode_noalloc,
     "rope": _rope,
     "rope_": _rope_inplace,
@@ -339,11 +337,12 @@ def _fake(*args, **kwargs) -> None:
 
 def _register() -> None:
     library = torch.library.Library(NAMESPACE, "DEF")
-    for name, schema in SCHEMAS.items():
+    schemas = SCHEMAS | MXFP4_SCHEMAS
+    for name, schema in schemas.items():
         library.define(schema)
         torch.library.register_fake(f"{NAMESPACE}::{name}", _fake, lib=library)
     missing = _load_native(NATIVE_LIBRARY)
-    for name in SCHEMAS:
+    for name in schemas:
         if name in KERNELS:
             library.impl(name, KERNELS[name], "CUDA")
         elif missing is not None:
