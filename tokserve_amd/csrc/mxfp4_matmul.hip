@@ -4,41 +4,12 @@
 // to the operands as they are stored. Lane 16 g + i holds row i and the g-th of four blocks;
 // which four blocks of K those are is free as long as A and B agree. Products of two codes
 // are exact in the accumulator; sums are fp32.
-#include "mxfp4_common.hpp"
+#include "mxfp4_matmul.hpp"
 
 #include <algorithm>
 
 namespace tks {
 namespace {
-
-typedef int mx_op __attribute__((ext_vector_type(8)));
-typedef float mx_f4 __attribute__((ext_vector_type(4)));
-
-// B . A^T of a 16-row tile each: D[4 g + r][i] with B's rows as the instruction's first
-// operand, so a lane holds four consecutive columns n of the output row m = i. The scale
-// bytes are byte SEL of sb and sa.
-template <int SEL>
-__device__ __forceinline__ mx_f4 mx_mfma(uint4 b, uint4 a, mx_f4 c, uint32_t sb, uint32_t sa) {
-#if __HIP_DEVICE_COMPILE__
-  // (e2m1, format 4, takes the first four registers of an operand.)
-  const mx_op x = {static_cast<int>(b.x), static_cast<int>(b.y), static_cast<int>(b.z),
-                   static_cast<int>(b.w), 0, 0, 0, 0};
-  const mx_op y = {static_cast<int>(a.x), static_cast<int>(a.y), static_cast<int>(a.z),
-                   static_cast<int>(a.w), 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, SEL, sb, SEL, sa);
-#else
-  (void)b; (void)a; (void)sb; (void)sa;
-  return c;
-#endif
-}
-
-struct MatmulArgs {
-  const uint8_t *a, *as;  // (M, K) codes and scale bytes, contiguous
-  const uint8_t *b, *bs;  // (N, K)
-  int64_t m, n, k;
-  void *out;
-  int64_t o_rs;
-};
 
 // ------------------------------------------------------------------------
 // Few rows: the weights stream from HBM straight to the operands.
@@ -126,7 +97,7 @@ __global__ __launch_bounds__(64 * kWaves) void matmul_few_kernel(MatmulArgs p) {
 }
 
 template <typename T>
-int32_t launch(const MatmulArgs &p, hipStream_t s) {
+int32_t launch_few(const MatmulArgs &p, hipStream_t s) {
   const int mt = static_cast<int>(std::min<int64_t>(4, ceil_div(p.m, 16)));
   const int64_t gx = ceil_div(p.n, 16), gy = ceil_div(p.m, 16 * mt);
   if (gx > 0x7fffffff || gy > 65535) return TKS_ERR_VALUE;
@@ -140,8 +111,20 @@ int32_t launch(const MatmulArgs &p, hipStream_t s) {
   return check_launch();
 }
 
-// Quantized activations in a workspace: codes, then scale bytes, each padded to 256 bytes.
-int64_t codes_bytes(int64_t m, int64_t k) { return ceil_div(m * k / 2, 256) * 256; }
+// The rows from which the tiled kernel is used, and the K its 32-bit offsets reach.
+constexpr int64_t kTileRows = 65;
+constexpr int64_t kTileDepth = int64_t{1} << 24;
+bool tiled(int64_t m, int64_t k) { return m >= kTileRows && k <= kTileDepth; }
+
+int32_t launch_few_of(const MatmulArgs &p, int32_t dtype, hipStream_t s) {
+  switch (dtype) {
+    case TKS_FLOAT32: return launch_few<float>(p, s);
+    case TKS_FLOAT16: return launch_few<_Float16>(p, s);
+    default: return launch_few<bf16_t>(p, s);
+  }
+}
+
+int64_t padded(int64_t bytes) { return ceil_div(bytes, 256) * 256; }
 
 constexpr int64_t kMaxDim = int64_t{1} << 40;
 
@@ -149,14 +132,21 @@ bool shape_ok(int64_t m, int64_t n, int64_t k) {
   return m >= 0 && n >= 0 && k > 0 && k % kMxBlock == 0 && m <= kMaxDim / k && n <= kMaxDim / k;
 }
 
+bool workspace_ok(const void *workspace, int64_t bytes, int64_t needed) {
+  return needed == 0 || (workspace != nullptr && aligned16(workspace) && bytes >= needed);
+}
+
 }  // namespace
 }  // namespace tks
 
 using namespace tks;
 
+// Both scales in window order, for the tiled kernel.
 extern "C" int64_t tks_mxfp4_matmul_workspace_bytes(int64_t num_rows, int64_t num_cols,
                                                     int64_t depth) {
-  return shape_ok(num_rows, num_cols, depth) ? 0 : -1;
+  if (!shape_ok(num_rows, num_cols, depth)) return -1;
+  if (!tiled(num_rows, depth) || num_cols == 0) return 0;
+  return padded(window_scale_bytes(num_rows, depth)) + window_scale_bytes(num_cols, depth);
 }
 
 extern "C" int32_t tks_mxfp4_matmul(const void *a_codes, const void *a_scales,
@@ -170,21 +160,33 @@ extern "C" int32_t tks_mxfp4_matmul(const void *a_codes, const void *a_scales,
   if (!a_codes || !a_scales || !b_codes || !b_scales || !out || !aligned16(a_codes) ||
       !aligned16(b_codes))
     return TKS_ERR_VALUE;
-  const MatmulArgs p{static_cast<const uint8_t *>(a_codes), static_cast<const uint8_t *>(a_scales),
-                     static_cast<const uint8_t *>(b_codes), static_cast<const uint8_t *>(b_scales),
-                     num_rows, num_cols, depth, out, out_row_stride};
+  if (!workspace_ok(workspace, workspace_bytes,
+                    tks_mxfp4_matmul_workspace_bytes(num_rows, num_cols, depth)))
+    return TKS_ERR_WORKSPACE;
+  MatmulArgs p{static_cast<const uint8_t *>(a_codes), static_cast<const uint8_t *>(a_scales),
+               static_cast<const uint8_t *>(b_codes), static_cast<const uint8_t *>(b_scales),
+               num_rows, num_cols, depth, out, out_row_stride};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  switch (dtype) {
-    case TKS_FLOAT32: return launch<float>(p, s);
-    case TKS_FLOAT16: return launch<_Float16>(p, s);
-    default: return launch<bf16_t>(p, s);
-  }
+  if (!tiled(num_rows, depth)) return launch_few_of(p, dtype, s);
+  uint8_t *as = static_cast<uint8_t *>(workspace);
+  uint8_t *bs = as + padded(window_scale_bytes(num_rows, depth));
+  int32_t st = launch_window_scales(p.as, num_rows, depth, as, s);
+  if (st == TKS_OK) st = launch_window_scales(p.bs, num_cols, depth, bs, s);
+  if (st != TKS_OK) return st;
+  p.as = as;
+  p.bs = bs;
+  return launch_matmul_tiles(p, dtype, s);
 }
 
+// The rows' codes and their scales (in window order for the tiled kernel, which takes the
+// weight's so too).
 extern "C" int64_t tks_mxfp4_linear_workspace_bytes(int64_t num_rows, int64_t num_cols,
                                                     int64_t depth) {
   if (!shape_ok(num_rows, num_cols, depth)) return -1;
-  return codes_bytes(num_rows, depth) + ceil_div(num_rows * (depth / kMxBlock), 256) * 256;
+  if (num_rows == 0 || num_cols == 0) return 0;
+  const int64_t codes = padded(num_rows * depth / 2);
+  if (!tiled(num_rows, depth)) return codes + num_rows * (depth / kMxBlock);
+  return codes + padded(window_scale_bytes(num_rows, depth)) + window_scale_bytes(num_cols, depth);
 }
 
 extern "C" int32_t tks_mxfp4_linear(const void *input, int64_t input_row_stride,
@@ -197,14 +199,24 @@ extern "C" int32_t tks_mxfp4_linear(const void *input, int64_t input_row_stride,
   if (num_rows == 0 || num_cols == 0) return TKS_OK;
   if (!input || !weight_codes || !weight_scales || !out || !aligned16(weight_codes))
     return TKS_ERR_VALUE;
-  if (workspace == nullptr || !aligned16(workspace) ||
-      workspace_bytes < tks_mxfp4_linear_workspace_bytes(num_rows, num_cols, depth))
+  if (!workspace_ok(workspace, workspace_bytes,
+                    tks_mxfp4_linear_workspace_bytes(num_rows, num_cols, depth)))
     return TKS_ERR_WORKSPACE;
+  hipStream_t s = static_cast<hipStream_t>(stream);
   uint8_t *codes = static_cast<uint8_t *>(workspace);
-  uint8_t *scales = codes + codes_bytes(num_rows, depth);
-  const int32_t st = tks_mxfp4_quantize(input, input_row_stride, num_rows, depth, codes, scales,
-                                        dtype, stream);
+  uint8_t *as = codes + padded(num_rows * depth / 2);
+  MatmulArgs p{codes, as, static_cast<const uint8_t *>(weight_codes),
+               static_cast<const uint8_t *>(weight_scales), num_rows, num_cols, depth, out,
+               out_row_stride};
+  if (!tiled(num_rows, depth)) {
+    const int32_t st = tks_mxfp4_quantize(input, input_row_stride, num_rows, depth, codes, as,
+                                          dtype, stream);
+    return st != TKS_OK ? st : launch_few_of(p, dtype, s);
+  }
+  uint8_t *bs = as + padded(window_scale_bytes(num_rows, depth));
+  const int32_t st = launch_quantize_windows(input, input_row_stride, num_rows, depth, codes, as,
+                                             p.bs, num_cols, bs, dtype, s);
   if (st != TKS_OK) return st;
-  return tks_mxfp4_matmul(codes, scales, weight_codes, weight_scales, num_rows, num_cols, depth,
-                          out, out_row_stride, nullptr, 0, dtype, stream);
+  p.bs = bs;
+  return launch_matmul_tiles(p, dtype, s);
 }
