@@ -1,17 +1,22 @@
 // The tiled MXFP4 product, for more rows than the weights' stream alone would pay for.
 //
-// A workgroup of 2 x 2 waves computes 32 MI x 32 NI of the output, a wave 16 MI x 16 NI: K in
-// steps of 128, one v_mfma_scale 16x16x128 per pair of 16-row tiles. A's codes go through LDS
-// (both waves of a row of waves read them), B's from L2 straight to the operands: either path
-// alone, LDS or the vector cache, would be the bound. Nothing is waited for in the step that
-// asks for it. In step s
-//   - A's codes of step s + 1 go from LDS to the operands of the next step,
-//   - those of step s + 2, in registers since step s - 1, go to LDS, and those of s + 3 are asked
-//     for in their place,
-//   - B's operands of step s + 1 are asked for,
-// while the matrix unit works on step s; a barrier ends it. The LDS ring has four slots and
-// the steps are unrolled by four: a scale dword holds a row's bytes of four steps (one window,
-// mxfp4_matmul.hpp), which the instruction picks its byte from.
+// A workgroup of 2 x 2 waves computes 32 MI x 32 NI of the output, a wave 16 MI x 16 NI: one
+// v_mfma_scale 16x16x128 per pair of 16-row tiles and 128 of K. Codes and scales go from L2 to
+// LDS without passing through registers, in units of 256 of K (128 bytes of a row: requests of
+// whole cache lines; in units of 128 the same loads reach half the rate, 31 against 60 bytes
+// per clock and CU), two units and the scales of two windows (mxfp4_matmul.hpp) at a time.
+//
+// A unit is two phases. While the matrix unit works on one, the operands of the next are read
+// from LDS: all of B's into a second set of registers, each of A's into the registers of the
+// one that was just used. So a unit's last LDS read is in its first phase, and in its second
+// its LDS is filled again, two units ahead, a few loads after each row of products. A barrier
+// per unit makes the next unit's codes visible and this one's LDS free.
+//
+// What bounds it: at 8192 x 8192 x 4096, 164 - 183 us (3.0 - 3.4 PFLOP/s), 155 without the
+// stores; of the matrix unit's nominal rate that is a third, of the rate that it keeps up in
+// this loop without loads (power: the clock falls) six tenths. Tiles of 256 x 256, one wave
+// per SIMD, take 186 us, since nothing covers a tile's first loads and its stores; two
+// workgroups of 128 x 128 per CU cover each other's.
 //
 // Past K the codes read are those of the last block, and both scales 2^-127, whose product
 // with any two codes is below the smallest fp32: adding it changes nothing.
@@ -41,144 +46,234 @@ __device__ __forceinline__ void tile_of(int64_t id, int64_t tiles_m, int64_t til
   *tn = in / rows;
 }
 
+// 16 bytes per lane from base + off to LDS address `to` (wave-uniform) + 16 * lane. As asm, so
+// that the compiler, which cannot tell the ring's slots apart, does not make every LDS read
+// wait for it: unit_barrier waits, and nothing else in the loop counts as such a load.
+__device__ __forceinline__ void load_lds_async(const uint8_t *base, uint32_t off, uint32_t to) {
+#if __HIP_DEVICE_COMPILE__
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(to)
+               : "memory", "m0");
+#else
+  (void)base; (void)off; (void)to;
+#endif
+}
+
+// The wave's loads into LDS are there, its LDS reads done, and so those of the others.
+__device__ __forceinline__ void unit_barrier() {
+#if __HIP_DEVICE_COMPILE__
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#endif
+}
+
+// mx_mfma<SEL> with the sum in place, in accumulation registers (left to itself the compiler
+// moves them about: 2048 x 11264 x 2048 36.8 -> 54.7 us).
+// The compiler does not see what the instruction needs around it: the wait states after a
+// VALU write of an operand are here, those before a VALU read of a sum are settle_sums.
+template <int SEL>
+__device__ __forceinline__ void mfma_in_place(uint4 b4, uint4 a4, mx_f4 &c, uint32_t sb,
+                                              uint32_t sa) {
+#if __HIP_DEVICE_COMPILE__
+  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+  const u4 b = {b4.x, b4.y, b4.z, b4.w}, a = {a4.x, a4.y, a4.z, a4.w};
+#define TKS_MFMA(sel)                                                                          \
+  asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 " sel                \
+      " cbsz:4 blgp:4"                                                                         \
+      : "+a"(c)                                                                                \
+      : "v"(b), "v"(a), "v"(sb), "v"(sa))
+  if constexpr (SEL == 0) TKS_MFMA("op_sel_hi:[0,0,0]");
+  if constexpr (SEL == 1) TKS_MFMA("op_sel:[1,1,0] op_sel_hi:[0,0,0]");
+  if constexpr (SEL == 2) TKS_MFMA("op_sel_hi:[1,1,0]");
+  if constexpr (SEL == 3) TKS_MFMA("op_sel:[1,1,0] op_sel_hi:[1,1,0]");
+#undef TKS_MFMA
+#else
+  (void)b4; (void)a4; (void)sb; (void)sa; (void)c;
+#endif
+}
+template <int MI, int NI>
+__device__ __forceinline__ void settle_sums(mx_f4 (&acc)[MI][NI]) {
+#if __HIP_DEVICE_COMPILE__
+  asm volatile("s_nop 15\n\ts_nop 15");
+#pragma unroll
+  for (int x = 0; x < MI; ++x)
+#pragma unroll
+    for (int y = 0; y < NI; ++y) asm volatile("" : "+a"(acc[x][y]));
+#endif
+}
+
+// Four floats as 16-bit T, packed.
+template <typename T>
+__device__ __forceinline__ uint2 four16(mx_f4 f) {
+  T t[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) t[r] = from_float<T>(f[r]);
+  uint2 v;
+  __builtin_memcpy(&v, t, 8);
+  return v;
+}
+// Of lane groups g, g + 1 (g even): the first gets both groups' v, the second both groups' w.
+__device__ __forceinline__ uint4 swap_halves(uint2 v, uint2 w) {
+#if __HIP_DEVICE_COMPILE__
+  const auto x = __builtin_amdgcn_permlane16_swap(v.x, w.x, false, false);
+  const auto y = __builtin_amdgcn_permlane16_swap(v.y, w.y, false, false);
+  return make_uint4(x[0], y[0], x[1], y[1]);
+#else
+  return make_uint4(v.x, v.y, w.x, w.y);
+#endif
+}
+
+__device__ __forceinline__ uint32_t lds_base(const void *p) {
+  return __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(
+      reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void *)p)));
+}
+
 template <typename T, int MI, int NI, bool VEC>
-__global__ __launch_bounds__(kThreads) void matmul_tiles_kernel(MatmulArgs p, int64_t tiles_m,
-                                                                int64_t tiles_n) {
-  constexpr int BM = 32 * MI, BN = 32 * NI;
-  constexpr int kSlots = 4;
-  constexpr int kStage = BM * 64 / 16 / kThreads;  // 16-byte pieces of an A step per thread
-  static_assert(kStage * 16 * kThreads == BM * 64, "whole pieces");
-  __shared__ __align__(16) uint8_t ring[kSlots][BM * 64];
+__global__ __launch_bounds__(kThreads, 1) void matmul_tiles_kernel(MatmulArgs p, int64_t tiles_m,
+                                                                   int64_t tiles_n) {
+  constexpr int BM = 32 * MI, BN = 32 * NI, kRows = BM + BN;
+  constexpr int kUnitBytes = kRows * 128;
+  constexpr int kLoads = kRows / 32;                // a wave's loads of a unit, 8 rows each
+  constexpr int kPart = (kLoads + MI - 1) / MI;     // of them after each row of products
+  constexpr int kScaleRows = (kRows + 255) & ~255;  // 64 rows to a load
+  __shared__ __align__(1024) uint8_t ring[2][kUnitBytes];
+  __shared__ __align__(1024) uint8_t scale_ring[2][kScaleRows * 16];
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int uw = __builtin_amdgcn_readfirstlane(wave);
   const int g = lane >> 4, i = lane & 15;
   const int wm = wave >> 1, wn = wave & 1;
+  const int row_bytes = static_cast<int>(p.k / 2);
+  const int blocks = static_cast<int>(p.k / kMxBlock);
+  const int wins = static_cast<int>(windows(p.k));
+
+  // In LDS the eight blocks of a row (of a unit) are permuted by its bits 1 to 3, so that the 16
+  // rows of an operand read fall on different banks. Load q of a wave is rows 8 (4 q + wave) and
+  // up: lane's row is lane / 8 of them, and its block the one whose place lane % 8 is.
+  const int load_block = (lane & 7) ^ ((lane >> 4) & 3) ^ ((wave & 1) << 2);
+  const int perm = (i >> 1) & 7;
+  const int place[2] = {16 * (g ^ perm), 16 * ((4 + g) ^ perm)};  // of a phase's block
+  const int read_a = (16 * MI * wm + i) * 128, read_b = (BM + 16 * NI * wn + i) * 128;
+  const int read_sa = (16 * MI * wm + i) * 16 + 4 * g;
+  const int read_sb = (BM + 16 * NI * wn + i) * 16 + 4 * g;
+  const uint32_t ring_at = lds_base(&ring[0][0]), scale_at = lds_base(&scale_ring[0][0]);
+
   int64_t tm, tn;
   tile_of(blockIdx.x, tiles_m, tiles_n, &tm, &tn);
   const int64_t m0 = tm * BM, n0 = tn * BN;
   const int last_m = static_cast<int>(min<int64_t>(p.m - m0, BM)) - 1;
   const int last_n = static_cast<int>(min<int64_t>(p.n - n0, BN)) - 1;
-  const int row_bytes = static_cast<int>(p.k / 2);
-  const int blocks = static_cast<int>(p.k / kMxBlock);
-  const int wins = static_cast<int>(windows(p.k));
-  const uint8_t *a = p.a + m0 * row_bytes;
-  const uint8_t *b = p.b + n0 * row_bytes;
-
-  // A's piece q of this thread: row t / 4 + 64 q, block t % 4 of the step. In LDS a row's four
-  // blocks are permuted by its bits 2 and 3, so that the 16 rows of an operand read touch all
-  // banks once.
-  uint32_t a_off[kStage];
-  int a_lds[kStage];
-  const int piece = threadIdx.x & 3;
+  const uint8_t *a = p.a + m0 * row_bytes, *b = p.b + n0 * row_bytes;
+  const uint8_t *as = p.as + m0 * 16, *bs = p.bs + n0 * 16;
+  uint32_t off[kLoads];
 #pragma unroll
-  for (int q = 0; q < kStage; ++q) {
-    const int row = (threadIdx.x >> 2) + 64 * q;
-    a_off[q] = static_cast<uint32_t>(min(row, last_m)) * row_bytes;
-    a_lds[q] = row * 64 + 16 * (piece ^ ((row >> 2) & 3));
+  for (int q = 0; q < kLoads; ++q) {
+    const int row = 8 * (4 * q + wave) + (lane >> 3);
+    off[q] = static_cast<uint32_t>(32 * q < BM ? min(row, last_m) : min(row - BM, last_n)) *
+             row_bytes;
   }
-  const int read_at = (16 * MI * wm + i) * 64 + 16 * (g ^ ((i >> 2) & 3));
-  uint32_t b_off[NI];
+  auto fetch = [&](int unit, int slot, int from, int to) {
+    const uint32_t at = 16u * static_cast<uint32_t>(min(8 * unit + load_block, blocks - 1));
 #pragma unroll
-  for (int t = 0; t < NI; ++t)
-    b_off[t] = static_cast<uint32_t>(min(16 * (NI * wn + t) + i, last_n)) * row_bytes;
-  // (Scales are padded to whole tiles of rows: those past the last are read and not used.)
-  const uint8_t *as = p.as + (m0 + 16 * MI * wm) * 16;
-  const uint8_t *bs = p.bs + (n0 + 16 * NI * wn) * 16;
-  const uint32_t s_off = 16 * i + 4 * g;
+    for (int q = 0; q < kLoads; ++q)
+      if (q >= from && q < to)
+        load_lds_async(32 * q < BM ? a : b, off[q] + at,
+                       ring_at + slot * kUnitBytes + (4 * q + uw) * 1024);
+  };
+  auto fetch_scales = [&](int win) {
+    const uint8_t *wa = as + win * (p.m * 16), *wb = bs + win * (p.n * 16);
+#pragma unroll
+    for (int q = 0; q < kScaleRows / 256; ++q) {
+      const int row = 64 * (4 * q + uw);  // (BM is a multiple of 64; rows past kRows: any)
+      const bool of_a = row < BM;
+      const int from = of_a ? row : min(row - BM, BN - 64);
+      load_lds_async(of_a ? wa : wb, static_cast<uint32_t>(16 * (from + lane)),
+                     scale_at + (win & 1) * (kScaleRows * 16) + row * 16);
+    }
+  };
 
-  uint4 stage[kStage], af[2][MI], bf[2][NI];
-  uint32_t sa[MI], sb[NI], sa_next[MI], sb_next[NI];
+  uint4 af[MI], bf[2][NI];
+  uint32_t sa[MI], sb[NI];
   mx_f4 acc[MI][NI];
+  auto get_scales = [&](int win) {
+    const uint8_t *s = scale_ring[win & 1];
+#pragma unroll
+    for (int t = 0; t < MI; ++t)
+      sa[t] = *reinterpret_cast<const uint32_t *>(s + read_sa + 256 * t);
+#pragma unroll
+    for (int t = 0; t < NI; ++t)
+      sb[t] = *reinterpret_cast<const uint32_t *>(s + read_sb + 256 * t);
+  };
+
+  fetch_scales(0);
+  fetch(0, 0, 0, kLoads);
+  fetch(1, 1, 0, kLoads);
+  const int units = 2 * wins;
 #pragma unroll
   for (int x = 0; x < MI; ++x)
 #pragma unroll
     for (int y = 0; y < NI; ++y) acc[x][y] = mx_f4{0.f, 0.f, 0.f, 0.f};
+  unit_barrier();
+  get_scales(0);
+#pragma unroll
+  for (int t = 0; t < NI; ++t) bf[0][t] = ld16(&ring[0][read_b + place[0] + 2048 * t]);
+#pragma unroll
+  for (int t = 0; t < MI; ++t) af[t] = ld16(&ring[0][read_a + place[0] + 2048 * t]);
 
-  auto fetch_a = [&](int step) {
-    const uint32_t at = 16u * static_cast<uint32_t>(min(4 * step + piece, blocks - 1));
-#pragma unroll
-    for (int q = 0; q < kStage; ++q) stage[q] = ld16(a + (a_off[q] + at));
-  };
-  auto put_a = [&](int slot) {
-#pragma unroll
-    for (int q = 0; q < kStage; ++q) st16(&ring[slot][a_lds[q]], stage[q]);
-  };
-  auto get_a = [&](int slot, uint4 *f) {
-#pragma unroll
-    for (int t = 0; t < MI; ++t) f[t] = ld16(&ring[slot][read_at + 1024 * t]);
-  };
-  auto fetch_b = [&](int step, uint4 *f) {
-    const uint32_t at = 16u * static_cast<uint32_t>(min(4 * step + g, blocks - 1));
-#pragma unroll
-    for (int t = 0; t < NI; ++t) f[t] = ld16(b + (b_off[t] + at));
-  };
-  auto fetch_scales = [&](uint32_t *xa, uint32_t *xb) {
-#pragma unroll
-    for (int t = 0; t < MI; ++t) xa[t] = *reinterpret_cast<const uint32_t *>(as + (s_off + 256 * t));
-#pragma unroll
-    for (int t = 0; t < NI; ++t) xb[t] = *reinterpret_cast<const uint32_t *>(bs + (s_off + 256 * t));
-  };
-
-  fetch_scales(sa, sb);
-  fetch_a(0);
-  put_a(0);
-  fetch_a(1);
-  fetch_b(0, bf[0]);
-  put_a(1);
-  fetch_a(2);
-  __syncthreads();
-  get_a(0, af[0]);
-
-#define TKS_STEP(T4)                                                                           \
+  // Phase T4 of a window: products of the operands at hand; those of the next phase, NEXT of
+  // the unit in SLOT, are read, and with FETCH unit `unit` goes to the other slot.
+#define TKS_PHASE(T4, SLOT, NEXT, FETCH)                                                       \
   {                                                                                            \
-    constexpr int cur = T4 & 1, nxt = cur ^ 1;                                                 \
-    get_a((T4 + 1) & 3, af[nxt]);                                                              \
-    fetch_b(step + T4 + 1, bf[nxt]);                                                           \
-    put_a((T4 + 2) & 3);                                                                       \
-    fetch_a(step + T4 + 3);                                                                    \
+    constexpr int cur = T4 & 1;                                                                \
+    const uint8_t *from = &ring[SLOT][place[NEXT]];                                            \
+    _Pragma("unroll") for (int t = 0; t < NI; ++t) bf[cur ^ 1][t] =                            \
+        ld16(from + read_b + 2048 * t);                                                        \
     _Pragma("unroll") for (int x = 0; x < MI; ++x) {                                           \
       _Pragma("unroll") for (int y = 0; y < NI; ++y)                                           \
-          acc[x][y] = mx_mfma<T4>(bf[cur][y], af[cur][x], acc[x][y], sb[y], sa[x]);            \
+          mfma_in_place<T4>(bf[cur][y], af[x], acc[x][y], sb[y], sa[x]);                       \
+      af[x] = ld16(from + read_a + 2048 * x);                                                  \
+      if (FETCH && unit < units) fetch(unit, SLOT ^ 1, kPart * x, kPart * x + kPart);          \
+      __builtin_amdgcn_sched_barrier(0);                                                       \
     }                                                                                          \
-    __syncthreads();                                                                           \
   }
   for (int win = 0; win < wins; ++win) {
-    if (win + 1 < wins) {
-      as += p.m * 16;
-      bs += p.n * 16;
-    }
-    fetch_scales(sa_next, sb_next);
-    const int step = 4 * win;
-    TKS_STEP(0)
-    TKS_STEP(1)
-    TKS_STEP(2)
-    TKS_STEP(3)
-#pragma unroll
-    for (int t = 0; t < MI; ++t) sa[t] = sa_next[t];
-#pragma unroll
-    for (int t = 0; t < NI; ++t) sb[t] = sb_next[t];
+    int unit = 2 * win + 2;
+    TKS_PHASE(0, 0, 1, false)
+    unit_barrier();
+    if (win + 1 < wins) fetch_scales(win + 1);
+    TKS_PHASE(1, 1, 0, true)
+    ++unit;
+    TKS_PHASE(2, 1, 1, false)
+    unit_barrier();
+    TKS_PHASE(3, 0, 0, true)
+    get_scales(win + 1);  // (after the last window: not used)
   }
-#undef TKS_STEP
+#undef TKS_PHASE
+  settle_sums<MI, NI>(acc);
 
   T *out = static_cast<T *>(p.out) + m0 * p.o_rs + n0;
 #pragma unroll
   for (int x = 0; x < MI; ++x) {
     const int row = 16 * (MI * wm + x) + i;
-    if (row > last_m) continue;
     T *o = out + row * p.o_rs;
 #pragma unroll
     for (int y = 0; y < NI; ++y) {
       const int col = 16 * (NI * wn + y) + 4 * g;
-      if constexpr (VEC) {
-        if (col > last_n) continue;
-        T v[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = from_float<T>(acc[x][y][r]);
-        __builtin_memcpy(__builtin_assume_aligned(o + col, 4 * sizeof(T)), v, sizeof(v));
+      if constexpr (VEC && sizeof(T) == 2) {
+        // Four columns are 8 bytes: lanes of neighbouring groups exchange halves of two column
+        // tiles, so that each stores 16 (2048 x 11264: 42.9 -> 39.3 us).
+        if (y & 1) continue;
+        const uint2 v = four16<T>(acc[x][y]), w = four16<T>(acc[x][y + 1]);
+        const uint4 both = swap_halves(v, w);
+        const int at = 16 * (NI * wn + y + (g & 1)) + 8 * (g >> 1);
+        if (row <= last_m && at <= last_n) st16(o + at, both);
+      } else if constexpr (VEC) {
+        const mx_f4 v = acc[x][y];
+        if (row <= last_m && col <= last_n)
+          st16(o + col, make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]),
+                                   __float_as_uint(v[2]), __float_as_uint(v[3])));
       } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (col + r <= last_n) o[col + r] = from_float<T>(acc[x][y][r]);
+          if (row <= last_m && col + r <= last_n) o[col + r] = from_float<T>(acc[x][y][r]);
       }
     }
   }
@@ -249,29 +344,32 @@ __global__ __launch_bounds__(kThreads) void quantize_windows_kernel(
 }
 
 template <typename T, int MI, int NI>
-void launch_tiles(const MatmulArgs &p, hipStream_t s) {
+int32_t launch_tiles(const MatmulArgs &p, hipStream_t s) {
   const int64_t tm = ceil_div(p.m, 32 * MI), tn = ceil_div(p.n, 32 * NI);
+  if (tm > 0x7fffffff / tn) return TKS_ERR_VALUE;
   const unsigned grid = static_cast<unsigned>(tm * tn);
-  const bool vec = p.n % 4 == 0 && p.o_rs % 4 == 0 &&
-                   reinterpret_cast<uintptr_t>(p.out) % (4 * sizeof(T)) == 0;
+  // (Whole 16-byte pieces of a row: eight 16-bit columns, four fp32.)
+  const bool vec = p.n * sizeof(T) % 16 == 0 && p.o_rs * sizeof(T) % 16 == 0 && aligned16(p.out);
   if (vec)
     matmul_tiles_kernel<T, MI, NI, true><<<grid, kThreads, 0, s>>>(p, tm, tn);
   else
     matmul_tiles_kernel<T, MI, NI, false><<<grid, kThreads, 0, s>>>(p, tm, tn);
+  return check_launch();
 }
 
+// The largest tiles that still give each CU enough of them. us at 128 x 128, 64 x 128 and
+// 64 x 64 (bf16):
+//   2048 x 11264 x 2048 (1,408 tiles of 128 x 128)  36.8, 49.3, 53.0
+//   1024 x 11264 x 2048 (704)                       23.3, 28.6, 28.3
+//   2048 x 2048 x 5632  (256)                       21.9, 20.4, 23.0
+//   300 x 11264 x 2048  (264; 440 of 64 x 128)      12.4, 10.0, 10.4
+//   777 x 2048 x 5632   (112; 208)                  16.1, 13.1, 12.6
+//   512 x 2048 x 2048   (64; 128)                   8.3, 6.6, 5.7
 template <typename T>
 int32_t launch(const MatmulArgs &p, hipStream_t s) {
-  if (ceil_div(p.m, 64) > 0x7fffffff / ceil_div(p.n, 64)) return TKS_ERR_VALUE;
-  const int64_t tiles = ceil_div(p.m, 256) * ceil_div(p.n, 256);
-  const int64_t half = ceil_div(p.m, 128) * ceil_div(p.n, 128);
-  if (tiles >= 200)
-    launch_tiles<T, 8, 8>(p, s);
-  else if (half >= 200)
-    launch_tiles<T, 4, 4>(p, s);
-  else
-    launch_tiles<T, 2, 2>(p, s);
-  return check_launch();
+  if (ceil_div(p.m, 128) * ceil_div(p.n, 128) >= 512) return launch_tiles<T, 4, 4>(p, s);
+  if (ceil_div(p.m, 64) * ceil_div(p.n, 128) >= 256) return launch_tiles<T, 2, 4>(p, s);
+  return launch_tiles<T, 2, 2>(p, s);
 }
 
 }  // namespace
