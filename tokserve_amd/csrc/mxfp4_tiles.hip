@@ -89,14 +89,11 @@ __device__ __forceinline__ void mfma_in_place(uint4 b4, uint4 a4, mx_f4 &c, uint
   (void)b4; (void)a4; (void)sb; (void)sa; (void)c;
 #endif
 }
-template <int MI, int NI>
-__device__ __forceinline__ void settle_sums(mx_f4 (&acc)[MI][NI]) {
+// (In the loop's last round, not after it: what the compiler moves between the loop's registers
+// and those of its exit comes right behind the loop.)
+__device__ __forceinline__ void settle_sums() {
 #if __HIP_DEVICE_COMPILE__
-  asm volatile("s_nop 15\n\ts_nop 15");
-#pragma unroll
-  for (int x = 0; x < MI; ++x)
-#pragma unroll
-    for (int y = 0; y < NI; ++y) asm volatile("" : "+a"(acc[x][y]));
+  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
 #endif
 }
 
@@ -244,10 +241,12 @@ __global__ __launch_bounds__(kThreads, 1) void matmul_tiles_kernel(MatmulArgs p,
     TKS_PHASE(2, 1, 1, false)
     unit_barrier();
     TKS_PHASE(3, 0, 0, true)
-    get_scales(win + 1);  // (after the last window: not used)
+    if (win + 1 < wins)
+      get_scales(win + 1);
+    else
+      settle_sums();
   }
 #undef TKS_PHASE
-  settle_sums<MI, NI>(acc);
 
   T *out = static_cast<T *>(p.out) + m0 * p.o_rs + n0;
 #pragma unroll
