@@ -68,23 +68,29 @@ def test_matrices_that_are_refused(fake) -> None:
         ops.mxfp4_quantize(fake(4, 64, dtype=torch.int32))
     with pytest.raises(TypeError, match="float4_e2m1fn_x2"):
         ops.mxfp4_dequantize(fake(4, 32, dtype=torch.uint8), scales, torch.float32)
-    with pytest.raises(TypeError, match="dtype must be"):
+    with pytest.raises(TypeError, match="out must be float32"):
         ops.mxfp4_dequantize(codes, scales, torch.float64)
     with pytest.raises(ValueError, match="one entry per 32"):
         ops.mxfp4_dequantize(codes, fake(4, 1, dtype=SCALES), torch.float32)
     with pytest.raises(ValueError, match="contiguous"):
         ops.mxfp4_dequantize(fake(8, 32, dtype=CODES)[::2], scales, torch.float32)
-    with pytest.raises(ValueError, match="with the inputs' K"):
+    with pytest.raises(ValueError, match="the inputs' K"):
         ops.mxfp4_linear(fake(3, 32), codes, scales)
-    with pytest.raises(ValueError, match="with A's K"):
+    with pytest.raises(ValueError, match="have A's K"):
         ops.mxfp4_matmul(codes, scales, fake(4, 16, dtype=CODES), fake(4, 1, dtype=SCALES),
                          torch.float32)
     with pytest.raises(ValueError, match="at least one row"):
         ops.mxfp4_linear(fake(3, 64), fake(0, 32, dtype=CODES), fake(0, 2, dtype=SCALES))
     with pytest.raises(ValueError, match="out must have shape"):
         ops.mxfp4_linear(fake(3, 64), codes, scales, out=fake(3, 5))
-    with pytest.raises(ValueError, match="out must have shape"):
+    with pytest.raises(ValueError, match="the inputs' dtype"):
         ops.mxfp4_linear(fake(3, 64), codes, scales, out=fake(3, 4, dtype=torch.float16))
+    with pytest.raises(ValueError, match="the given dtype"):
+        ops.mxfp4_dequantize(codes, scales, torch.float16, out=fake(4, 64))
+    with pytest.raises(ValueError, match="go together"):
+        ops.mxfp4_quantize(fake(4, 64), codes=codes)
+    with pytest.raises(ValueError, match="shape \\(..., K / 2\\)"):
+        ops.mxfp4_quantize(fake(3, 64), codes=codes, scales=scales)
     with pytest.raises(ValueError, match="must be contiguous"):
         ops.mxfp4_linear(fake(3, 2, 64), codes, scales, out=fake(3, 2, 8)[..., :4])
     with pytest.raises(ValueError, match="workspace must be"):

@@ -146,6 +146,18 @@ __device__ __forceinline__ uint32_t mx_quantize(const MxEight<T> &x, uint32_t *s
   return mx_codes<T>(x, *scale_byte);
 }
 
+// Quantizes a block that the lane holds alone: its 16 bytes of codes and its scale byte.
+template <typename T>
+__device__ __forceinline__ uint4 mx_quantize_block(const MxEight<T> (&x)[4],
+                                                   uint32_t *scale_byte) {
+  uint32_t m = mx_largest<T>(x[0]);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) m = max(m, mx_largest<T>(x[i]));
+  *scale_byte = mx_scale_byte(mx_exponent<T>(m));
+  return make_uint4(mx_codes<T>(x[0], *scale_byte), mx_codes<T>(x[1], *scale_byte),
+                    mx_codes<T>(x[2], *scale_byte), mx_codes<T>(x[3], *scale_byte));
+}
+
 // Codes 2 SEL and 2 SEL + 1 of a word times the scale, as floats.
 template <int SEL>
 __device__ __forceinline__ void mx_pair(uint32_t codes, float scale, float *out) {

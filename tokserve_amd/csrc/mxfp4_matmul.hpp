@@ -53,8 +53,9 @@ inline int64_t window_scale_bytes(int64_t rows, int64_t k) {
 
 // The tiled product over A's and B's codes and window-ordered scales (16-byte aligned).
 int32_t launch_matmul_tiles(const MatmulArgs &p, int32_t dtype, hipStream_t s);
-// Scale bytes (rows, k / 32) into window order.
-int32_t launch_window_scales(const uint8_t *scales, int64_t rows, int64_t k, uint8_t *out,
+// A's and B's scale bytes (rows, k / 32) into window order.
+int32_t launch_window_scales(const uint8_t *a_scales, int64_t m, uint8_t *a_out,
+                             const uint8_t *b_scales, int64_t n, uint8_t *b_out, int64_t k,
                              hipStream_t s);
 // Rows of `dtype` to codes and window-ordered scales, and B's scales (n, k / 32) into window
 // order, in one launch.

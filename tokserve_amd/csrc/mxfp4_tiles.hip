@@ -295,11 +295,15 @@ __device__ __forceinline__ void window_scales(const uint8_t *scales, int64_t row
   st16(out + item * 16, make_uint4(v[0], v[1], v[2], v[3]));
 }
 
-__global__ __launch_bounds__(kThreads) void window_scales_kernel(const uint8_t *scales,
-                                                                 int64_t rows, int64_t blocks,
-                                                                 int64_t total, uint8_t *out) {
+__global__ __launch_bounds__(kThreads) void window_scales_kernel(
+    const uint8_t *a_scales, int64_t m, uint8_t *a_out, const uint8_t *b_scales, int64_t n,
+    uint8_t *b_out, int64_t blocks) {
+  const int64_t w = windows(blocks * kMxBlock);
   const int64_t item = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (item < total) window_scales(scales, rows, blocks, item, out);
+  if (item < m * w)
+    window_scales(a_scales, m, blocks, item, a_out);
+  else if (item < (m + n) * w)
+    window_scales(b_scales, n, blocks, item - m * w, b_out);
 }
 
 // The first `quant` workgroups quantize (a thread eight values, kItems times), the others put
@@ -381,12 +385,13 @@ int32_t launch_matmul_tiles(const MatmulArgs &p, int32_t dtype, hipStream_t s) {
   }
 }
 
-int32_t launch_window_scales(const uint8_t *scales, int64_t rows, int64_t k, uint8_t *out,
+int32_t launch_window_scales(const uint8_t *a_scales, int64_t m, uint8_t *a_out,
+                             const uint8_t *b_scales, int64_t n, uint8_t *b_out, int64_t k,
                              hipStream_t s) {
-  const int64_t total = rows * windows(k);
-  if (ceil_div(total, kThreads) > 0x7fffffff) return TKS_ERR_VALUE;
-  window_scales_kernel<<<static_cast<unsigned>(ceil_div(total, kThreads)), kThreads, 0, s>>>(
-      scales, rows, k / kMxBlock, total, out);
+  const int64_t grid = ceil_div((m + n) * windows(k), kThreads);
+  if (grid > 0x7fffffff) return TKS_ERR_VALUE;
+  window_scales_kernel<<<static_cast<unsigned>(grid), kThreads, 0, s>>>(
+      a_scales, m, a_out, b_scales, n, b_out, k / kMxBlock);
   return check_launch();
 }
 

@@ -25,6 +25,7 @@
 #include <dlfcn.h>
 
 #include <atomic>
+#include <initializer_list>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -453,52 +454,158 @@ void silu_mul(const Tensor &gate_up, const Tensor &out) {
         "silu_mul");
 }
 
+// The MXFP4 matrix operators check their arguments here (torch_ops.py does the same for
+// traced calls): in Python the checks of a small product took 5 us of its 12.6.
+bool is_float(const Tensor &t) {
+  return t.scalar_type() == at::kFloat || t.scalar_type() == at::kHalf ||
+         t.scalar_type() == at::kBFloat16;
+}
+
+void one_device(const char *op, const Tensor &first, std::initializer_list<const Tensor *> others) {
+  TORCH_CHECK_VALUE(first.is_cuda(), op, " requires HIP device tensors");
+  for (const Tensor *t : others) {
+    if (t == nullptr) continue;
+    TORCH_CHECK_VALUE(t->is_cuda(), op, " requires HIP device tensors");
+    TORCH_CHECK_VALUE(t->device() == first.device(), op, ": tensors must use the same device");
+  }
+}
+
+bool same_lead(const Tensor &a, const Tensor &b) {
+  return a.dim() == b.dim() && a.sizes().slice(0, a.dim() - 1) == b.sizes().slice(0, b.dim() - 1);
+}
+
+int64_t float_depth(const char *op, const Tensor &t, const char *name) {
+  TORCH_CHECK_TYPE(is_float(t), op, ": ", name, " must be float32, float16 or bfloat16");
+  const int64_t depth = t.dim() ? t.size(-1) : 0;
+  TORCH_CHECK_VALUE(depth >= 1 && depth % 32 == 0, op, ": the last dimension of ", name,
+                    " must be a positive multiple of 32");
+  return depth;
+}
+
+int64_t mxfp4_depth(const char *op, const Tensor &codes, const Tensor &scales, const char *name) {
+  TORCH_CHECK_TYPE(codes.scalar_type() == at::kFloat4_e2m1fn_x2 &&
+                       scales.scalar_type() == at::kFloat8_e8m0fnu,
+                   op, ": ", name, " codes must be float4_e2m1fn_x2 and scales float8_e8m0fnu");
+  const int64_t half = codes.dim() ? codes.size(-1) : 0;
+  TORCH_CHECK_VALUE(half >= 1 && half % 16 == 0, op, ": ", name,
+                    " must hold a positive multiple of 32 values a row");
+  TORCH_CHECK_VALUE(same_lead(codes, scales) && scales.size(-1) == half / 16, op, ": ", name,
+                    " scales must have one entry per 32 values");
+  TORCH_CHECK_VALUE(codes.is_contiguous() && scales.is_contiguous(), op, ": ", name,
+                    " codes and scales must be contiguous");
+  return 2 * half;
+}
+
+int64_t weight_depth(const char *op, const Tensor &codes, const Tensor &scales, const char *name) {
+  TORCH_CHECK_VALUE(codes.dim() == 2 && codes.size(0) >= 1, op, ": ", name,
+                    " must have shape (N, K) and at least one row");
+  return mxfp4_depth(op, codes, scales, name);
+}
+
+void check_rows_out(const char *op, const Tensor &out, const Tensor &rows, int64_t width) {
+  TORCH_CHECK_VALUE(same_lead(out, rows) && out.size(-1) == width &&
+                        (out.numel() == 0 || out.stride(-1) == 1),
+                    op, ": out must have shape (..., ", width, ") after the rows', its last "
+                    "dimension contiguous");
+  TORCH_CHECK_VALUE(out.dim() == 2 || out.is_contiguous(), op,
+                    ": an out of other than two dimensions must be contiguous");
+}
+
+void check_space(const char *op, const OptTensor &workspace) {
+  TORCH_CHECK_VALUE(!workspace || (workspace->scalar_type() == at::kByte &&
+                                   workspace->is_contiguous()),
+                    op, ": workspace must be a contiguous uint8 tensor");
+}
+
+const Tensor *maybe(const OptTensor &t) { return t ? &*t : nullptr; }
+
+// Rows and row stride of a matrix whose last dimension is `width` long and contiguous (of
+// other than two dimensions: contiguous).
+int64_t rows_of(const Tensor &t, int64_t width) {
+  return t.dim() == 2 ? t.size(0) : t.numel() / width;
+}
+int64_t row_stride(const Tensor &t, int64_t width) { return t.dim() == 2 ? t.stride(0) : width; }
+// The input as such a matrix, copied where it is not one.
+Tensor as_rows(const Tensor &t) {
+  return t.dim() == 2 ? (t.stride(1) == 1 ? t : t.contiguous()) : t.contiguous();
+}
+
 void mxfp4_quantize(const Tensor &input, const Tensor &codes, const Tensor &scales) {
+  const char *op = "mxfp4_quantize";
+  one_device(op, input, {&codes, &scales});
+  const int64_t depth = float_depth(op, input, "inputs");
+  TORCH_CHECK_VALUE(mxfp4_depth(op, codes, scales, "output") == depth && same_lead(codes, input),
+                    op, ": codes must have shape (..., K / 2)");
   const c10::DeviceGuard guard(input.device());
-  check(library().tks_mxfp4_quantize(input.const_data_ptr(), input.stride(0), input.size(0),
-                                     input.size(1), codes.mutable_data_ptr(),
-                                     scales.mutable_data_ptr(), code(input), stream_of(input)),
-        "mxfp4_quantize");
+  const Tensor x = as_rows(input);
+  check(library().tks_mxfp4_quantize(x.const_data_ptr(), row_stride(x, depth), rows_of(x, depth),
+                                     depth, codes.mutable_data_ptr(), scales.mutable_data_ptr(),
+                                     code(x), stream_of(x)),
+        op);
 }
 
 void mxfp4_dequantize(const Tensor &codes, const Tensor &scales, const Tensor &out) {
+  const char *op = "mxfp4_dequantize";
+  one_device(op, codes, {&scales, &out});
+  TORCH_CHECK_TYPE(is_float(out), op, ": out must be float32, float16 or bfloat16");
+  const int64_t depth = mxfp4_depth(op, codes, scales, "input");
+  check_rows_out(op, out, codes, depth);
   const c10::DeviceGuard guard(codes.device());
   check(library().tks_mxfp4_dequantize(codes.const_data_ptr(), scales.const_data_ptr(),
-                                       out.size(0), out.size(1), out.mutable_data_ptr(),
-                                       out.stride(0), code(out), stream_of(out)),
-        "mxfp4_dequantize");
+                                       rows_of(out, depth), depth, out.mutable_data_ptr(),
+                                       row_stride(out, depth), code(out), stream_of(out)),
+        op);
 }
 
 void mxfp4_matmul(const Tensor &a_codes, const Tensor &a_scales, const Tensor &b_codes,
                   const Tensor &b_scales, const Tensor &out, const OptTensor &workspace) {
+  const char *op = "mxfp4_matmul";
+  one_device(op, a_codes, {&a_scales, &b_codes, &b_scales, &out, maybe(workspace)});
+  TORCH_CHECK_TYPE(is_float(out), op, ": out must be float32, float16 or bfloat16");
+  const int64_t depth = mxfp4_depth(op, a_codes, a_scales, "A");
+  TORCH_CHECK_VALUE(weight_depth(op, b_codes, b_scales, "B") == depth, op, ": B must have A's K");
+  const int64_t width = b_codes.size(0);
+  check_rows_out(op, out, a_codes, width);
+  check_space(op, workspace);
   const c10::DeviceGuard guard(a_codes.device());
   const Library &l = library();
-  const int64_t m = a_codes.size(0), n = b_codes.size(0), k = 2 * a_codes.size(1);
+  const int64_t rows = rows_of(out, width);
   const Tensor ws = workspace ? *workspace
-                              : scratch(l.tks_mxfp4_matmul_workspace_bytes(m, n, k), out,
-                                        "mxfp4_matmul");
+                              : scratch(l.tks_mxfp4_matmul_workspace_bytes(rows, width, depth),
+                                        out, op);
   check(l.tks_mxfp4_matmul(a_codes.const_data_ptr(), a_scales.const_data_ptr(),
-                           b_codes.const_data_ptr(), b_scales.const_data_ptr(), m, n, k,
-                           out.mutable_data_ptr(), out.stride(0),
+                           b_codes.const_data_ptr(), b_scales.const_data_ptr(), rows, width, depth,
+                           out.mutable_data_ptr(), row_stride(out, width),
                            ws.defined() ? ws.mutable_data_ptr() : nullptr,
                            ws.defined() ? ws.numel() : 0, code(out), stream_of(out)),
-        "mxfp4_matmul");
+        op);
 }
 
 void mxfp4_linear(const Tensor &input, const Tensor &weight_codes, const Tensor &weight_scales,
                   const Tensor &out, const OptTensor &workspace) {
+  const char *op = "mxfp4_linear";
+  one_device(op, input, {&weight_codes, &weight_scales, &out, maybe(workspace)});
+  const int64_t depth = float_depth(op, input, "inputs");
+  TORCH_CHECK_VALUE(out.scalar_type() == input.scalar_type(), op,
+                    ": out must have the inputs' dtype");
+  TORCH_CHECK_VALUE(weight_depth(op, weight_codes, weight_scales, "the weight") == depth, op,
+                    ": the weight must have the inputs' K");
+  const int64_t width = weight_codes.size(0);
+  check_rows_out(op, out, input, width);
+  check_space(op, workspace);
   const c10::DeviceGuard guard(input.device());
   const Library &l = library();
-  const int64_t m = input.size(0), n = weight_codes.size(0), k = input.size(1);
+  const Tensor x = as_rows(input);
+  const int64_t rows = rows_of(x, depth);
   const Tensor ws = workspace ? *workspace
-                              : scratch(l.tks_mxfp4_linear_workspace_bytes(m, n, k), out,
-                                        "mxfp4_linear");
-  check(l.tks_mxfp4_linear(input.const_data_ptr(), input.stride(0),
-                           weight_codes.const_data_ptr(), weight_scales.const_data_ptr(), m, n, k,
-                           out.mutable_data_ptr(), out.stride(0),
+                              : scratch(l.tks_mxfp4_linear_workspace_bytes(rows, width, depth), x,
+                                        op);
+  check(l.tks_mxfp4_linear(x.const_data_ptr(), row_stride(x, depth), weight_codes.const_data_ptr(),
+                           weight_scales.const_data_ptr(), rows, width, depth,
+                           out.mutable_data_ptr(), row_stride(out, width),
                            ws.defined() ? ws.mutable_data_ptr() : nullptr,
-                           ws.defined() ? ws.numel() : 0, code(input), stream_of(input)),
-        "mxfp4_linear");
+                           ws.defined() ? ws.numel() : 0, code(x), stream_of(x)),
+        op);
 }
 
 }  // namespace

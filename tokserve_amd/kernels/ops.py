@@ -24,7 +24,11 @@ _ops = torch.ops.tokserve_amd
 def require_hip(operation: str, *tensors: torch.Tensor) -> torch.device:
     """All tensors on one HIP device (torch reports HIP tensors as is_cuda)."""
 
+    # (device indices cost a third of is_cuda and device, a microsecond of a small call)
+    index = tensors[0].get_device()
     device = tensors[0].device
+    if index >= 0 and device.type == "cuda" and all([t.get_device() == index for t in tensors]):
+        return device
     for tensor in tensors:
         if not tensor.is_cuda:
             raise ValueError(f"{operation} requires HIP device tensors")
@@ -119,7 +123,8 @@ def _row_scales(
         raise ValueError(f"{operation}: k_scales and v_scales go together")
     if mxfp4:
         require_hip(operation, key_cache, k_scales, v_scales)
-        shape = (*key_cache.shape[:4], 2 * key_cache.shape[4] // MXFP4_BLOCK)
+        *shape, half = key_cache.shape
+        shape = (*shape, 2 * half // MXFP4_BLOCK)
         for name, scales in (("k_scales", k_scales), ("v_scales", v_scales)):
             if scales.dtype != MXFP4_SCALE_DTYPE:
                 raise TypeError(f"{name} of MXFP4 pools must be float8_e8m0fnu")
@@ -481,51 +486,8 @@ def paged_attention_prefill(
 # MXFP4 matrices
 
 
-def _float_rows(operation: str, tensor: torch.Tensor, name: str) -> torch.Tensor:
-    """(..., K) float values as rows (R, K), K contiguous and whole MXFP4 blocks."""
-
-    if tensor.dtype not in (torch.float32, torch.float16, torch.bfloat16):
-        raise TypeError(f"{operation}: {name} must be float32, float16 or bfloat16")
-    if tensor.ndim < 1 or tensor.shape[-1] < 1 or tensor.shape[-1] % MXFP4_BLOCK != 0:
-        raise ValueError(f"{operation}: the last dimension of {name} must be a positive multiple "
-                         "of 32")
-    # (numel is 0 without rows, where -1 could not be inferred)
-    rows = tensor.reshape(tensor.numel() // tensor.shape[-1], tensor.shape[-1])
-    return _last_dim_contiguous(rows, name)
-
-
-def _mxfp4_operand(operation: str, codes: torch.Tensor, scales: torch.Tensor, name: str) -> int:
-    """Checks one MXFP4 tensor, codes (..., K / 2) and scales (..., K / 32); returns K."""
-
-    require_hip(operation, codes, scales)
-    if codes.dtype != MXFP4_DTYPE or scales.dtype != MXFP4_SCALE_DTYPE:
-        raise TypeError(f"{operation}: {name} codes must be float4_e2m1fn_x2 and scales "
-                        "float8_e8m0fnu")
-    depth = 2 * codes.shape[-1] if codes.ndim else 0
-    if depth < 1 or depth % MXFP4_BLOCK != 0:
-        raise ValueError(f"{operation}: {name} must hold a positive multiple of 32 values a row")
-    if scales.shape != (*codes.shape[:-1], depth // MXFP4_BLOCK):
-        raise ValueError(f"{operation}: {name} scales must have one entry per 32 values")
-    if not codes.is_contiguous() or not scales.is_contiguous():
-        raise ValueError(f"{operation}: {name} codes and scales must be contiguous")
-    return depth
-
-
-def _product_out(operation: str, like: torch.Tensor, shape: tuple[int, ...], dtype: torch.dtype,
-                 out: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor]:
-    """The output (given or new) and its rows."""
-
-    if out is None:
-        out = torch.empty(shape, dtype=dtype, device=like.device)
-    require_hip(operation, like, out)
-    if out.shape != shape or out.dtype != dtype or (out.numel() and out.stride(-1) != 1):
-        raise ValueError(f"{operation}: out must have shape {tuple(shape)} and the dtype {dtype}, "
-                         "its last dimension contiguous")
-    if out.ndim == 2:
-        return out, out
-    if not out.is_contiguous():
-        raise ValueError(f"{operation}: an out of more than two dimensions must be contiguous")
-    return out, out.view(out.numel() // shape[-1], shape[-1])
+# (Shapes, dtypes and devices are checked by the operators themselves, natively on the device
+# and in Python while tracing: a small product takes about as long as its host side.)
 
 
 def mxfp4_quantize(
@@ -537,19 +499,15 @@ def mxfp4_quantize(
     """(..., K) values to MXFP4: codes (..., K / 2) float4_e2m1fn_x2 and scales (..., K / 32)
     float8_e8m0fnu, blocks of 32 along the last dimension (K a multiple of 32)."""
 
-    require_hip("mxfp4_quantize", inputs)
-    rows = _float_rows("mxfp4_quantize", inputs, "inputs")
-    lead, depth = inputs.shape[:-1], inputs.shape[-1]
-    if codes is None:
-        codes = torch.empty((*lead, depth // 2), dtype=MXFP4_DTYPE, device=inputs.device)
-    if scales is None:
+    device = require_hip("mxfp4_quantize", inputs)
+    if codes is None and scales is None:
+        *lead, depth = inputs.shape if inputs.ndim else (0,)
+        codes = torch.empty((*lead, depth // 2), dtype=MXFP4_DTYPE, device=device)
         scales = torch.empty((*lead, depth // MXFP4_BLOCK), dtype=MXFP4_SCALE_DTYPE,
-                             device=inputs.device)
-    require_hip("mxfp4_quantize", inputs, codes)
-    if codes.shape != (*lead, depth // 2):
-        raise ValueError("mxfp4_quantize: codes must have shape (..., K / 2)")
-    _mxfp4_operand("mxfp4_quantize", codes, scales, "output")
-    _ops.mxfp4_quantize(rows, codes, scales)
+                             device=device)
+    elif codes is None or scales is None:
+        raise ValueError("mxfp4_quantize: codes and scales go together")
+    _ops.mxfp4_quantize(inputs, codes, scales)
     return codes, scales
 
 
@@ -563,11 +521,13 @@ def mxfp4_dequantize(
     """The values (..., K) of codes (..., K / 2) and scales (..., K / 32), rounded to dtype
     (exact in float32 and bfloat16)."""
 
-    depth = _mxfp4_operand("mxfp4_dequantize", codes, scales, "input")
-    if dtype not in (torch.float32, torch.float16, torch.bfloat16):
-        raise TypeError("mxfp4_dequantize: dtype must be float32, float16 or bfloat16")
-    out, rows = _product_out("mxfp4_dequantize", codes, (*codes.shape[:-1], depth), dtype, out)
-    _ops.mxfp4_dequantize(codes, scales, rows)
+    device = require_hip("mxfp4_dequantize", codes)
+    if out is None:
+        *lead, half = codes.shape if codes.ndim else (0,)
+        out = torch.empty((*lead, 2 * half), dtype=dtype, device=device)
+    elif out.dtype != dtype:
+        raise ValueError("mxfp4_dequantize: out must have the given dtype")
+    _ops.mxfp4_dequantize(codes, scales, out)
     return out
 
 
@@ -588,19 +548,13 @@ def mxfp4_matmul(
     one must be ordered on one stream. It is allocated when it is not given.
     """
 
-    depth = _mxfp4_operand("mxfp4_matmul", a_codes, a_scales, "A")
-    if b_codes.ndim != 2 or _mxfp4_operand("mxfp4_matmul", b_codes, b_scales, "B") != depth:
-        raise ValueError("mxfp4_matmul: B must have shape (N, K) with A's K")
-    require_hip("mxfp4_matmul", a_codes, b_codes)
-    if b_codes.shape[0] < 1:
-        raise ValueError("mxfp4_matmul: B must have at least one row")
-    if dtype not in (torch.float32, torch.float16, torch.bfloat16):
-        raise TypeError("mxfp4_matmul: dtype must be float32, float16 or bfloat16")
-    out, rows = _product_out("mxfp4_matmul", a_codes, (*a_codes.shape[:-1], b_codes.shape[0]),
-                             dtype, out)
-    _check_workspace("mxfp4_matmul", a_codes, workspace)
-    _ops.mxfp4_matmul(a_codes.view(rows.shape[0], depth // 2), a_scales,
-                      b_codes, b_scales, rows, workspace)
+    device = require_hip("mxfp4_matmul", a_codes)
+    if out is None:
+        out = torch.empty((*a_codes.shape[:-1], b_codes.shape[0] if b_codes.ndim else 0),
+                          dtype=dtype, device=device)
+    elif out.dtype != dtype:
+        raise ValueError("mxfp4_matmul: out must have the given dtype")
+    _ops.mxfp4_matmul(a_codes, a_scales, b_codes, b_scales, out, workspace)
     return out
 
 
@@ -618,18 +572,11 @@ def mxfp4_linear(
     results are those of the two calls. `workspace` as there, of mxfp4_linear_workspace_bytes.
     """
 
-    require_hip("mxfp4_linear", inputs, weight_codes)
-    rows_in = _float_rows("mxfp4_linear", inputs, "inputs")
-    if (weight_codes.ndim != 2
-            or _mxfp4_operand("mxfp4_linear", weight_codes, weight_scales, "weight")
-            != inputs.shape[-1]):
-        raise ValueError("mxfp4_linear: the weight must have shape (N, K) with the inputs' K")
-    if weight_codes.shape[0] < 1:
-        raise ValueError("mxfp4_linear: the weight must have at least one row")
-    out, rows = _product_out("mxfp4_linear", inputs, (*inputs.shape[:-1], weight_codes.shape[0]),
-                             inputs.dtype, out)
-    _check_workspace("mxfp4_linear", inputs, workspace)
-    _ops.mxfp4_linear(rows_in, weight_codes, weight_scales, rows, workspace)
+    device = require_hip("mxfp4_linear", inputs)
+    if out is None:
+        out = torch.empty((*inputs.shape[:-1], weight_codes.shape[0] if weight_codes.ndim else 0),
+                          dtype=inputs.dtype, device=device)
+    _ops.mxfp4_linear(inputs, weight_codes, weight_scales, out, workspace)
     return out
 
 

@@ -330,9 +330,114 @@ def _unavailable(reason: str):
 
 
 def _fake(*args, **kwargs) -> None:
-    """Every operator writes only into tensors it is given: nothing to propagate."""
+    """Operators write only into tensors they are given: nothing to propagate."""
 
     return None
+
+
+# The MXFP4 matrix operators check their own arguments: csrc/torch_ops.cpp on the device, and
+# their fake kernels, with the same conditions and messages, while tracing.
+MXFP4_SCALE_DTYPE = torch.float8_e8m0fnu
+_FLOAT_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _one_device(operation: str, *tensors: torch.Tensor | None) -> None:
+    given = [t for t in tensors if t is not None]
+    if any(not t.is_cuda for t in given):
+        raise ValueError(f"{operation} requires HIP device tensors")
+    if len({t.device for t in given}) > 1:
+        raise ValueError(f"{operation}: tensors must use the same device")
+
+
+def _float_depth(operation: str, tensor: torch.Tensor, name: str) -> int:
+    if tensor.dtype not in _FLOAT_DTYPES:
+        raise TypeError(f"{operation}: {name} must be float32, float16 or bfloat16")
+    depth = tensor.shape[-1] if tensor.ndim else 0
+    if depth < 1 or depth % 32 != 0:
+        raise ValueError(f"{operation}: the last dimension of {name} must be a positive multiple "
+                         "of 32")
+    return depth
+
+
+def _mxfp4_depth(operation: str, codes: torch.Tensor, scales: torch.Tensor, name: str) -> int:
+    """Values in a row of an MXFP4 tensor, codes (..., K / 2) and scales (..., K / 32)."""
+
+    if codes.dtype != MXFP4_POOL_DTYPE or scales.dtype != MXFP4_SCALE_DTYPE:
+        raise TypeError(f"{operation}: {name} codes must be float4_e2m1fn_x2 and scales "
+                        "float8_e8m0fnu")
+    half = codes.shape[-1] if codes.ndim else 0
+    if half < 1 or half % 16 != 0:
+        raise ValueError(f"{operation}: {name} must hold a positive multiple of 32 values a row")
+    if scales.shape != (*codes.shape[:-1], half // 16):
+        raise ValueError(f"{operation}: {name} scales must have one entry per 32 values")
+    if not codes.is_contiguous() or not scales.is_contiguous():
+        raise ValueError(f"{operation}: {name} codes and scales must be contiguous")
+    return 2 * half
+
+
+def _check_rows_out(operation: str, out: torch.Tensor, lead: torch.Size, width: int) -> None:
+    if out.shape != (*lead, width) or (out.numel() and out.stride(-1) != 1):
+        raise ValueError(f"{operation}: out must have shape (..., {width}) after the rows', its "
+                         "last dimension contiguous")
+    if out.ndim != 2 and not out.is_contiguous():
+        raise ValueError(f"{operation}: an out of other than two dimensions must be contiguous")
+
+
+def _check_space(operation: str, workspace: torch.Tensor | None) -> None:
+    if workspace is not None and (workspace.dtype != torch.uint8 or not workspace.is_contiguous()):
+        raise ValueError(f"{operation}: workspace must be a contiguous uint8 tensor")
+
+
+def _weight_depth(operation: str, codes: torch.Tensor, scales: torch.Tensor, name: str) -> int:
+    if codes.ndim != 2 or codes.shape[0] < 1:
+        raise ValueError(f"{operation}: {name} must have shape (N, K) and at least one row")
+    return _mxfp4_depth(operation, codes, scales, name)
+
+
+def _fake_mxfp4_quantize(input, codes, scales) -> None:
+    _one_device("mxfp4_quantize", input, codes, scales)
+    depth = _float_depth("mxfp4_quantize", input, "inputs")
+    if (_mxfp4_depth("mxfp4_quantize", codes, scales, "output") != depth
+            or codes.shape[:-1] != input.shape[:-1]):
+        raise ValueError("mxfp4_quantize: codes must have shape (..., K / 2)")
+
+
+def _fake_mxfp4_dequantize(codes, scales, out) -> None:
+    _one_device("mxfp4_dequantize", codes, scales, out)
+    if out.dtype not in _FLOAT_DTYPES:
+        raise TypeError("mxfp4_dequantize: out must be float32, float16 or bfloat16")
+    depth = _mxfp4_depth("mxfp4_dequantize", codes, scales, "input")
+    _check_rows_out("mxfp4_dequantize", out, codes.shape[:-1], depth)
+
+
+def _fake_mxfp4_matmul(a_codes, a_scales, b_codes, b_scales, out, workspace=None) -> None:
+    _one_device("mxfp4_matmul", a_codes, a_scales, b_codes, b_scales, out, workspace)
+    if out.dtype not in _FLOAT_DTYPES:
+        raise TypeError("mxfp4_matmul: out must be float32, float16 or bfloat16")
+    depth = _mxfp4_depth("mxfp4_matmul", a_codes, a_scales, "A")
+    if _weight_depth("mxfp4_matmul", b_codes, b_scales, "B") != depth:
+        raise ValueError("mxfp4_matmul: B must have A's K")
+    _check_rows_out("mxfp4_matmul", out, a_codes.shape[:-1], b_codes.shape[0])
+    _check_space("mxfp4_matmul", workspace)
+
+
+def _fake_mxfp4_linear(input, weight_codes, weight_scales, out, workspace=None) -> None:
+    _one_device("mxfp4_linear", input, weight_codes, weight_scales, out, workspace)
+    depth = _float_depth("mxfp4_linear", input, "inputs")
+    if out.dtype != input.dtype:
+        raise ValueError("mxfp4_linear: out must have the inputs' dtype")
+    if _weight_depth("mxfp4_linear", weight_codes, weight_scales, "the weight") != depth:
+        raise ValueError("mxfp4_linear: the weight must have the inputs' K")
+    _check_rows_out("mxfp4_linear", out, input.shape[:-1], weight_codes.shape[0])
+    _check_space("mxfp4_linear", workspace)
+
+
+FAKES = {
+    "mxfp4_quantize": _fake_mxfp4_quantize,
+    "mxfp4_dequantize": _fake_mxfp4_dequantize,
+    "mxfp4_matmul": _fake_mxfp4_matmul,
+    "mxfp4_linear": _fake_mxfp4_linear,
+}
 
 
 def _register() -> None:
@@ -340,7 +445,7 @@ def _register() -> None:
     schemas = SCHEMAS | MXFP4_SCHEMAS
     for name, schema in schemas.items():
         library.define(schema)
-        torch.library.register_fake(f"{NAMESPACE}::{name}", _fake, lib=library)
+        torch.library.register_fake(f"{NAMESPACE}::{name}", FAKES.get(name, _fake), lib=library)
     missing = _load_native(NATIVE_LIBRARY)
     for name in schemas:
         if name in KERNELS:
