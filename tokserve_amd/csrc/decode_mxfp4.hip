@@ -23,8 +23,18 @@
 //
 // The softmax is online, in the log2 domain, with a lazy reference: a wave rescales its sums
 // when some score passes the reference by more than 8 (2^8 is harmless in bf16 and fp32).
+//
+// What bounds it is reading the pools, and the waits for them: a tile's loads are issued a tile
+// ahead, from an address that the wave holds in scalar registers (its pages are looked up 32
+// tiles at a time) and 32-bit lane offsets. bf16, 256 sequences of 128-8,192 keys (about 2,000
+// on average), Dh 128, 8 KV heads of 4 query heads each: 110 us, 5.2 TB/s; with each lane's
+// address in 64 bits and every tile waited for as soon as asked for: 212 us. fp16, 128
+// sequences of 0-1,152 keys, Dh 64, 4 KV heads of 8 query heads each: 11 us (18), most of it
+// the launch and the longest sequence's chain of tiles.
 #include "attention_common.hpp"
 #include "mxfp4_kv.hpp"
+
+#include <type_traits>
 
 namespace tks {
 namespace {
@@ -32,6 +42,7 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr float kSlack = 8.f;
+constexpr int kLookUp = 32;  // tiles whose pages a wave looks up at once
 
 typedef Mfma<bf16_t> Bf;
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -95,39 +106,45 @@ struct Tile {
   uint8_t vs[2][4][VB];
 };
 
-// The share of lane (g, i) of K row `row` and of V row `row`; c = i.
+// Byte offsets of lane (g, i)'s shares in a K and a V row.
 template <int NB>
-__device__ __forceinline__ void load_k(const uint8_t *codes, const uint8_t *scales, int64_t row,
-                                       int g, uint32_t *k, uint8_t *ks) {
-  const uint8_t *p = codes + row * (16 * NB) + 4 * NB * g;
-  __builtin_memcpy(k, __builtin_assume_aligned(p, NB == 4 ? 16 : NB == 2 ? 8 : 4), 4 * NB);
-  const uint8_t *s = scales + row * NB;
+__device__ __forceinline__ uint32_t k_share(int g) { return 4 * NB * g; }
+template <int NB>
+__device__ __forceinline__ uint32_t v_share(int i) {
+  return NB == 4 ? 4 * i : NB == 2 ? 2 * i : i;
+}
+// The share of K and V rows at p, their scale bytes at s (rows from `row` on).
+template <int NB>
+__device__ __forceinline__ void load_k(const uint8_t *p, const uint8_t *s, uint32_t row, int g,
+                                       uint32_t *k, uint8_t *ks) {
+  __builtin_memcpy(k, __builtin_assume_aligned(p + (row * (16 * NB) + k_share<NB>(g)),
+                                               NB == 4 ? 16 : NB == 2 ? 8 : 4),
+                   4 * NB);
   if constexpr (NB == 3) {
 #pragma unroll
-    for (int j = 0; j < 3; ++j) ks[j] = s[(3 * g + j) >> 2];
+    for (int j = 0; j < 3; ++j) ks[j] = s[row * NB + ((3 * g + j) >> 2)];
   } else {
-    ks[0] = s[g * NB / 4];
+    ks[0] = s[row * NB + g * NB / 4];
   }
 }
 template <int NB>
-__device__ __forceinline__ void load_v(const uint8_t *codes, const uint8_t *scales, int64_t row,
-                                       int c, uint32_t *v, uint8_t *vs) {
-  const uint8_t *p = codes + row * (16 * NB);
-  const uint8_t *s = scales + row * NB;
+__device__ __forceinline__ void load_v(const uint8_t *p, const uint8_t *s, uint32_t row, int c,
+                                       uint32_t *v, uint8_t *vs) {
+  const uint32_t at = row * (16 * NB) + v_share<NB>(c);
   if constexpr (NB == 4) {
-    v[0] = *reinterpret_cast<const uint32_t *>(p + 4 * c);
-    vs[0] = s[c >> 2];
+    v[0] = *reinterpret_cast<const uint32_t *>(p + at);
+    vs[0] = s[row * NB + (c >> 2)];
   } else if constexpr (NB == 2) {
-    v[0] = *reinterpret_cast<const uint16_t *>(p + 2 * c);
-    vs[0] = s[c >> 3];
+    v[0] = *reinterpret_cast<const uint16_t *>(p + at);
+    vs[0] = s[row * NB + (c >> 3)];
   } else if constexpr (NB == 1) {
-    v[0] = p[c];
-    vs[0] = s[0];
+    v[0] = p[at];
+    vs[0] = s[row];
   } else {
 #pragma unroll
     for (int j = 0; j < 3; ++j) {
-      v[j] = p[c + 16 * j];
-      vs[j] = s[j];
+      v[j] = p[at + 16 * j];
+      vs[j] = s[row * NB + j];
     }
   }
 }
@@ -139,14 +156,15 @@ __device__ __forceinline__ int dim_of(int i, int jj) {
 
 // PAGED16: blocks of a multiple of 16 tokens; a half tile then lies in one block.
 template <typename T, int NB, bool PAGED16>
-__global__ __launch_bounds__(kThreads) void decode_mx_kernel(MxDecodeArgs a) {
+__global__ __launch_bounds__(kThreads, 2) void decode_mx_kernel(MxDecodeArgs a) {
   constexpr int DH = 32 * NB;
   constexpr int P = Parts<T>::N;
   constexpr int J = 2 * NB;  // P.V products: 16 dims each
   __shared__ float m_s[kWaves][16], l_s[kWaves][16];
   __shared__ __align__(16) float acc_s[kWaves][16][DH];
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, i = lane & 15;
   const int kvh = blockIdx.x, split = blockIdx.z;
   const int b = a.seq_order ? a.seq_order[blockIdx.y] : static_cast<int>(blockIdx.y);
@@ -165,15 +183,22 @@ __global__ __launch_bounds__(kThreads) void decode_mx_kernel(MxDecodeArgs a) {
   const int32_t *bt = a.bt + static_cast<int64_t>(b) * a.bt_stride;
   const int BS = a.kc.block_size;
 
-  // The query as the B operand of Q.K: head i (none past the group), dims of group g.
+  // The query as the B operand of Q.K: head i (zeros past the group), dims of group g.
   Bf::v8 q[P][NB];
+  const T *q_row = static_cast<const T *>(a.q) + b * a.q_ss +
+                   (static_cast<int64_t>(kvh) * G + min(i, G - 1)) * a.q_hs + 8 * NB * g;
+  MxEight<T> raw[NB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j)
+    raw[j] = a.q_vec ? mx_load8<T>(q_row + 8 * j) : mx_load8_any<T>(q_row + 8 * j);
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
     float x[8];
-    const T *src = static_cast<const T *>(a.q) + b * a.q_ss +
-                   (static_cast<int64_t>(kvh) * G + i) * a.q_hs + 8 * (NB * g + j);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = i < G ? to_float(src[e]) : 0.f;
+    for (int e = 0; e < static_cast<int>(sizeof(T) / 2); ++e)
+      unpack<T>(raw[j].v[e], x + e * Vec<T>::N);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = i < G ? x[e] : 0.f;
     Bf::v8 parts[P];
     split_parts<P>(x, parts);
 #pragma unroll
@@ -186,23 +211,44 @@ __global__ __launch_bounds__(kThreads) void decode_mx_kernel(MxDecodeArgs a) {
     const int page = key / BS;
     return a.kc.row(block_of(bt, page, a.kc.num_blocks), kvh, key - page * BS);
   };
+  // With PAGED16 a half tile is a page of 16 rows, id = pool row / 16 (of this layer): lane 2 n + h
+  // holds that of half h of the wave's tile `from` + n, so that a table entry is read long before
+  // its keys are.
+  int pages = 0;
+  auto look_up = [&](int from) {
+    const int key = begin + 32 * (wave + kWaves * (from + (lane >> 1))) + 16 * (lane & 1);
+    if (key < end) {
+      const int page = key / BS;
+      const int64_t block = block_of(bt, page, a.kc.num_blocks);
+      pages = static_cast<int>((block * a.kc.num_kv_heads + kvh) * (BS >> 4)) +
+              ((key - page * BS) >> 4);
+    }
+  };
+  const int64_t layer_row = a.kc.layer_base * BS;
   const int k_row = 4 * (i & 3) + (i >> 2);  // key of A row i of a half tile
-  auto load = [&](int tile, Tile<NB> &t) {
-    const int base = begin + 32 * tile;
+  auto load = [&](int n, Tile<NB> &t) {
+    const int base = begin + 32 * (wave + kWaves * n);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       if constexpr (PAGED16) {
-        const int64_t row = row_of(base + 16 * h) & ~int64_t{15};
-        load_k<NB>(a.kc.codes, a.kc.scales, row + k_row, g, t.k[h], t.ks[h]);
+        // (A page's address in scalar registers, the lane's part of it 32 bits.)
+        const int64_t row =
+            layer_row + 16 * static_cast<int64_t>(__builtin_amdgcn_readlane(
+                                 pages, 2 * (n & (kLookUp - 1)) + h));
+        const uint8_t *kp = a.kc.codes + row * (16 * NB), *ks = a.kc.scales + row * NB;
+        const uint8_t *vp = a.vc.codes + row * (16 * NB), *vs = a.vc.scales + row * NB;
+        load_k<NB>(kp, ks, k_row, g, t.k[h], t.ks[h]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          load_v<NB>(a.vc.codes, a.vc.scales, row + 4 * r + g, i, t.v[h][r], t.vs[h][r]);
+        for (int r = 0; r < 4; ++r) load_v<NB>(vp, vs, 4 * r + g, i, t.v[h][r], t.vs[h][r]);
       } else {
-        load_k<NB>(a.kc.codes, a.kc.scales, row_of(base + 16 * h + k_row), g, t.k[h], t.ks[h]);
+        const int64_t k_at = row_of(base + 16 * h + k_row);
+        load_k<NB>(a.kc.codes + k_at * (16 * NB), a.kc.scales + k_at * NB, 0, g, t.k[h], t.ks[h]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          load_v<NB>(a.vc.codes, a.vc.scales, row_of(base + 16 * h + 4 * r + g), i, t.v[h][r],
+        for (int r = 0; r < 4; ++r) {
+          const int64_t at = row_of(base + 16 * h + 4 * r + g);
+          load_v<NB>(a.vc.codes + at * (16 * NB), a.vc.scales + at * NB, 0, i, t.v[h][r],
                      t.vs[h][r]);
+        }
       }
     }
   };
@@ -212,8 +258,9 @@ __global__ __launch_bounds__(kThreads) void decode_mx_kernel(MxDecodeArgs a) {
 #pragma unroll
   for (int jj = 0; jj < J; ++jj) acc[jj] = Bf::f4{0.f, 0.f, 0.f, 0.f};
 
-  auto process = [&](const Tile<NB> &t, int base) {
-    const bool whole = base + 32 <= end;
+  // whole_tile: all 32 keys of the tile are the sequence's.
+  auto process = [&](const Tile<NB> &t, int base, auto whole_tile) {
+    constexpr bool whole = decltype(whole_tile)::value;
     float s[8];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -276,15 +323,38 @@ __global__ __launch_bounds__(kThreads) void decode_mx_kernel(MxDecodeArgs a) {
     }
   };
 
-  // The next tile's loads are in flight while one is worked on.
-  if (wave < tiles) {
-    Tile<NB> cur, next;
-    load(wave, cur);
-    for (int tile = wave; tile < tiles; tile += kWaves) {
-      if (tile + kWaves < tiles) load(tile + kWaves, next);
-      process(cur, begin + 32 * tile);
-      cur = next;
+  // The next tile's loads are in flight while one is worked on. Only the split's last tile may
+  // be a part of one; its wave works on it after the others of its own.
+  const int mine = (tiles - wave + kWaves - 1) / kWaves;
+  const int whole = (end - begin) / 32 > wave ? ((end - begin) / 32 - wave + kWaves - 1) / kWaves : 0;
+  if (mine > 0) {
+    Tile<NB> even, odd;
+    int looked_up = 0;
+    // (Past the last tile the last one again: were the loads in a branch, a tile's would all
+    // have to be waited for before the next one is worked on.)
+    auto fetch = [&](int n, Tile<NB> &t) {
+      n = min(n, mine - 1);
+      if constexpr (PAGED16)
+        if (n >= looked_up + kLookUp) look_up(looked_up += kLookUp);
+      load(n, t);
+    };
+    auto base_of = [&](int n) { return begin + 32 * (wave + kWaves * n); };
+    if constexpr (PAGED16) look_up(0);
+    load(0, even);
+    int n = 0;
+    for (; n + 1 < whole; n += 2) {
+      fetch(n + 1, odd);
+      process(even, base_of(n), std::true_type{});
+      fetch(n + 2, even);
+      process(odd, base_of(n + 1), std::true_type{});
     }
+    if (n < whole) {
+      fetch(n + 1, odd);
+      process(even, base_of(n), std::true_type{});
+      even = odd;
+      ++n;
+    }
+    if (n < mine) process(even, base_of(n), std::false_type{});
   }
   l = xgroup_sum(l);
 

@@ -65,6 +65,7 @@ int32_t launch_decode_mx_pages(const MxPool &kc, const MxPool &vc, const int32_t
 struct MxDecodeArgs {
   const void *q;
   int64_t q_ss, q_hs;
+  bool q_vec;  // query rows can be read 16 bytes at a time
   MxPool kc, vc;
   const int32_t *bt;
   int32_t bt_stride;

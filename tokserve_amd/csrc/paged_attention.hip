@@ -1224,6 +1224,8 @@ int32_t decode_mxfp4_impl(const void *query, int64_t q_seq_stride, int64_t q_hea
   a.q = query;
   a.q_ss = q_seq_stride;
   a.q_hs = q_head_stride;
+  const int elem = elem_bytes(dtype);
+  a.q_vec = aligned16(query) && q_seq_stride * elem % 16 == 0 && q_head_stride * elem % 16 == 0;
   a.kc = mx_pool(const_cast<void *>(key_cache), const_cast<void *>(k_scales), num_blocks,
                  num_kv_heads, block_size, head_dim, layer_index);
   a.vc = mx_pool(const_cast<void *>(value_cache), const_cast<void *>(v_scales), num_blocks,
