@@ -17,6 +17,7 @@ from tokserve_amd.kernels import ops
 pytestmark = pytest.mark.gpu
 
 DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+CODES, SCALES = torch.float4_e2m1fn_x2, torch.float8_e8m0fnu
 
 
 def _bytes(x: torch.Tensor) -> torch.Tensor:
@@ -210,3 +211,46 @@ def test_refused_products(device) -> None:
                                                                  device=device))
     with pytest.raises(ValueError, match="requires HIP device"):
         ops.mxfp4_linear(x, codes, scales, out=torch.empty(4, 40))
+
+
+def test_refused_matrices(device) -> None:
+    """The refusals of tests/test_mxfp4_host.py, by the operators themselves."""
+
+    def on(*shape, dtype=torch.float32):
+        return torch.zeros(shape, dtype=torch.uint8 if dtype.itemsize == 1 else dtype,
+                           device=device).view(dtype)
+
+    codes, scales = on(4, 32, dtype=CODES), on(4, 2, dtype=SCALES)
+    with pytest.raises(ValueError, match="multiple of 32"):
+        ops.mxfp4_quantize(on(4, 48))
+    with pytest.raises(TypeError, match="float32, float16 or bfloat16"):
+        ops.mxfp4_quantize(on(4, 64, dtype=torch.int32))
+    with pytest.raises(TypeError, match="float4_e2m1fn_x2"):
+        ops.mxfp4_dequantize(on(4, 32, dtype=torch.uint8), scales, torch.float32)
+    with pytest.raises(TypeError, match="out must be float32"):
+        ops.mxfp4_dequantize(codes, scales, torch.float64)
+    with pytest.raises(ValueError, match="one entry per 32"):
+        ops.mxfp4_dequantize(codes, on(4, 1, dtype=SCALES), torch.float32)
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.mxfp4_dequantize(on(8, 32, dtype=CODES)[::2], scales, torch.float32)
+    with pytest.raises(ValueError, match="the inputs' K"):
+        ops.mxfp4_linear(on(3, 32), codes, scales)
+    with pytest.raises(ValueError, match="have A's K"):
+        ops.mxfp4_matmul(codes, scales, on(4, 16, dtype=CODES), on(4, 1, dtype=SCALES),
+                         torch.float32)
+    with pytest.raises(ValueError, match="at least one row"):
+        ops.mxfp4_linear(on(3, 64), on(0, 32, dtype=CODES), on(0, 2, dtype=SCALES))
+    with pytest.raises(ValueError, match="out must have shape"):
+        ops.mxfp4_linear(on(3, 64), codes, scales, out=on(3, 5))
+    with pytest.raises(ValueError, match="the inputs' dtype"):
+        ops.mxfp4_linear(on(3, 64), codes, scales, out=on(3, 4, dtype=torch.float16))
+    with pytest.raises(ValueError, match="the given dtype"):
+        ops.mxfp4_dequantize(codes, scales, torch.float16, out=on(4, 64))
+    with pytest.raises(ValueError, match="go together"):
+        ops.mxfp4_quantize(on(4, 64), codes=codes)
+    with pytest.raises(ValueError, match="shape \\(..., K / 2\\)"):
+        ops.mxfp4_quantize(on(3, 64), codes=codes, scales=scales)
+    with pytest.raises(ValueError, match="must be contiguous"):
+        ops.mxfp4_linear(on(3, 2, 64), codes, scales, out=on(3, 2, 8)[..., :4])
+    with pytest.raises(ValueError, match="workspace must be"):
+        ops.mxfp4_linear(on(3, 64), codes, scales, workspace=on(100))

@@ -178,3 +178,29 @@ def test_c_entries_check_before_any_launch() -> None:
     assert decode(*args(pages=1)) == space
     assert library.tks_paged_attention_prefill_mxfp4_workspace_bytes(2, 1, 64, 16, 40, 0) == \
         2 * (2 * 3 * 16 * 64 * 4) + 256
+
+
+def test_projections_on_the_cpu() -> None:
+    from tokserve_amd.engine.config import LlamaConfig
+    from tokserve_amd.engine.layers import MXFP4Linear
+    from tokserve_amd.engine.model import LlamaModel
+
+    module = MXFP4Linear(64, 10)
+    assert module.codes.shape == (10, 32) and module.scales.shape == (10, 2)
+    assert module.bfloat16().codes.dtype == torch.uint8
+    assert list(module.state_dict()) == ["codes", "scales"]
+    with pytest.raises(ValueError, match="multiple of 32"):
+        MXFP4Linear(48, 10)
+    with pytest.raises(ValueError, match="out_features"):
+        MXFP4Linear(32, 0)
+    with pytest.raises(ValueError, match="requires HIP device"):
+        module(torch.zeros(1, 64))
+    sizes = dict(vocab_size=50, num_hidden_layers=1, num_attention_heads=2,
+                 num_key_value_heads=1, max_position_embeddings=64)
+    with pytest.raises(ValueError, match="hidden_size to be a multiple of 32"):
+        LlamaModel(LlamaConfig(hidden_size=40, intermediate_size=64, **sizes)).quantize_mxfp4()
+    model = LlamaModel(LlamaConfig(hidden_size=64, intermediate_size=96, **sizes))
+    with pytest.raises(ValueError, match="requires HIP device"):
+        model.quantize_mxfp4()
+    assert model.weights_version == 0
+    assert isinstance(model.layers[0].mlp.up_proj, torch.nn.Linear)

@@ -86,6 +86,7 @@ class DecodeGraphs:
         self.width_quantum = width_quantum
         self.max_graphs = max_graphs
         self._graphs: dict[tuple[int, int], _Captured] = {}
+        self._weights_version = getattr(model, "weights_version", 0)
         self._staging: list[torch.Tensor | None] = [None, None]
         self._staged: list[torch.cuda.Event | None] = [None, None]
         self._turn = 0
@@ -180,6 +181,12 @@ class DecodeGraphs:
         w = self.width_for(works)
         key = (b, w)
         host = self._host_bytes(works, w)
+        version = getattr(self.model, "weights_version", 0)
+        if self._weights_version != version:
+            # Graphs of weights that the model holds no longer.
+            torch.cuda.synchronize(self.device)
+            self._graphs.clear()
+            self._weights_version = version
         captured = self._graphs.get(key)
         if captured is not None:
             self._upload(host, captured.static, b, token_source)

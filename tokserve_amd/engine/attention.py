@@ -19,11 +19,10 @@ from typing import TYPE_CHECKING
 
 import torch
 from torch import nn
-from torch.nn import functional
 
 from tokserve_amd.engine.config import LlamaConfig
 from tokserve_amd.engine.kernel_backend import KernelBackend, check_backend
-from tokserve_amd.engine.layers import fused_weight
+from tokserve_amd.engine.layers import fused_linear, fused_weight
 from tokserve_amd.kernels import ops
 from tokserve_amd.kernels.paged_attention import hip_paged_attention
 from tokserve_amd.kernels.rope import hip_apply_rope
@@ -142,7 +141,8 @@ class GroupedQueryAttention(nn.Module):
 
         tokens = inputs.shape[0]
         hq, hkv, dh = self.num_attention_heads, self.num_key_value_heads, self.head_dim
-        qkv = functional.linear(inputs, self.qkv_weight())  # (N, (Hq + 2 Hkv) Dh)
+        qkv = fused_linear(self, [self.q_proj, self.k_proj, self.v_proj], "_qkv",
+                           inputs)  # (N, (Hq + 2 Hkv) Dh)
         query = qkv[:, : hq * dh].view(tokens, hq, dh)
         key = qkv[:, hq * dh : (hq + hkv) * dh].view(tokens, hkv, dh)
         value = qkv[:, (hq + hkv) * dh :].view(tokens, hkv, dh)
@@ -159,7 +159,7 @@ class GroupedQueryAttention(nn.Module):
                 **storage.scales)
             return self.o_proj(attended.view(tokens, self.hidden_size))
         # Q rotated in place; rotated K and V go straight to the pool slots (quantized
-        # with the pool scales over fp8 pools).
+        # with the pool scales over fp8 pools, block by block over MXFP4 ones).
         ops.rope_kv_append(query, key, value, batch.positions, rotary, storage.key_storage,
                            storage.value_storage, batch.slot_mapping, layer_index,
                            **storage.scales)
