@@ -454,8 +454,8 @@ int32_t tks_mxfp4_matmul(const void *a_codes, const void *a_scales, const void *
                          int64_t workspace_bytes, int32_t dtype, tks_stream_t stream);
 
 /* A projection with MXFP4 weights: rows of `dtype` are quantized as
- * tks_mxfp4_quantize does and multiplied as tks_mxfp4_matmul does; same results as
- * the two calls. Workspace as for the product, from its own size query. */
+ * tks_mxfp4_quantize does and multiplied as tks_mxfp4_matmul does; the results are the
+ * two calls' up to the order of their fp32 sums. Workspace as for the product, from its own size query. */
 int64_t tks_mxfp4_linear_workspace_bytes(int64_t num_rows, int64_t num_cols, int64_t depth);
 
 int32_t tks_mxfp4_linear(const void *input, int64_t input_row_stride, const void *weight_codes,

@@ -254,3 +254,34 @@ def test_refused_matrices(device) -> None:
         ops.mxfp4_linear(on(3, 2, 64), codes, scales, out=on(3, 2, 8)[..., :4])
     with pytest.raises(ValueError, match="workspace must be"):
         ops.mxfp4_linear(on(3, 64), codes, scales, workspace=on(100))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", [(65, 64, 2048), (100, 130, 2080), (128, 257, 5632), (190, 72, 2592),
+                                   (66, 1000, 4128), (40, 8200, 1056), (64, 8192, 2048)])
+def test_products_of_a_long_depth_or_many_columns(device, dtype, m, n, k) -> None:
+    """The projection and the two calls may sum in different orders here: each by itself."""
+
+    x = _rows(m, k, dtype, m + k, spread=4)
+    w = _rows(n, k, torch.float32, n + k, spread=3)
+    w_codes, w_scales = ops.mxfp4_quantize(w.to(device))
+    a = mxfp4.values(*mxfp4.quantize(x))
+    b = mxfp4.values(*mxfp4.quantize(w))
+    _check_product(ops.mxfp4_linear(x.to(device), w_codes, w_scales), a, b, dtype)
+    x_codes, x_scales = ops.mxfp4_quantize(x.to(device))
+    _check_product(ops.mxfp4_matmul(x_codes, x_scales, w_codes, w_scales, dtype), a, b, dtype)
+
+
+@pytest.mark.parametrize("m,k", [(70, 2080), (200, 5632)])
+def test_nan_blocks_of_a_long_depth(device, m, k) -> None:
+    """A NaN block makes its row (of A) or column (of B) NaN and nothing else."""
+
+    x = _rows(m, k, torch.float32, 3, spread=2)
+    w = _rows(96, k, torch.float32, 4, spread=2)
+    x[5, k - 1] = float("nan")
+    w[90, 1024] = float("inf")
+    out = ops.mxfp4_linear(x.to(device), *ops.mxfp4_quantize(w.to(device))).cpu()
+    bad = torch.zeros(m, 96, dtype=torch.bool)
+    bad[5] = True
+    bad[:, 90] = True
+    assert torch.equal(out.isnan(), bad)

@@ -17,7 +17,8 @@ namespace {
 
 // One workgroup per 16 columns of the output and 16 MT rows of it, its waves taking chunks of
 // 512 of K in turn, four blocks of its row a lane; their
-// sums meet in LDS, in wave order. With ROWS the activations come as they are and each lane
+// sums meet in LDS, in wave order. (With a chunk's loads issued a chunk ahead: no faster but for
+// one row of a long K, 11008 -> 4096 13.0 -> 9.6 us, and 16 rows 4096 -> 8192 8.3 -> 9.4.) With ROWS the activations come as they are and each lane
 // quantizes the four blocks it needs: all the workgroups do that work again, a fraction of a
 // microsecond of it, and a launch is saved.
 constexpr int kChunk = 512;
@@ -175,12 +176,15 @@ int32_t launch_few_mt(const FewArgs &f, hipStream_t s) {
 
 template <typename T, bool ROWS>
 int32_t launch_few(const FewArgs &f, hipStream_t s) {
-  if constexpr (ROWS) return launch_few_mt<T, 1, ROWS>(f, s);
-  switch (std::min<int64_t>(4, ceil_div(f.p.m, 16))) {
-    case 1: return launch_few_mt<T, 1, ROWS>(f, s);
-    case 2: return launch_few_mt<T, 2, ROWS>(f, s);
-    case 3: return launch_few_mt<T, 3, ROWS>(f, s);
-    default: return launch_few_mt<T, 4, ROWS>(f, s);
+  if constexpr (ROWS) {
+    return launch_few_mt<T, 1, ROWS>(f, s);
+  } else {
+    switch (std::min<int64_t>(4, ceil_div(f.p.m, 16))) {
+      case 1: return launch_few_mt<T, 1, ROWS>(f, s);
+      case 2: return launch_few_mt<T, 2, ROWS>(f, s);
+      case 3: return launch_few_mt<T, 3, ROWS>(f, s);
+      default: return launch_few_mt<T, 4, ROWS>(f, s);
+    }
   }
 }
 

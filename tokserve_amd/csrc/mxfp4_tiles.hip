@@ -18,6 +18,8 @@
 // per SIMD, take 186 us, since nothing covers a tile's first loads and its stores; two
 // workgroups of 128 x 128 per CU cover each other's.
 //
+// With few tiles a workgroup is four such groups of waves (below).
+//
 // Past K the codes read are those of the last block, and both scales 2^-127, whose product
 // with any two codes is below the smallest fp32: adding it changes nothing.
 #include "mxfp4_matmul.hpp"
@@ -123,19 +125,26 @@ __device__ __forceinline__ uint32_t lds_base(const void *p) {
       reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void *)p)));
 }
 
-template <typename T, int MI, int NI, bool VEC>
-__global__ __launch_bounds__(kThreads, 1) void matmul_tiles_kernel(MatmulArgs p, int64_t tiles_m,
-                                                                   int64_t tiles_n) {
+// GROUPS: sets of 2 x 2 waves that take the windows of K in turn, each with LDS of its own;
+// their sums meet in LDS, in the groups' order.
+template <typename T, int MI, int NI, int GROUPS, bool VEC>
+__global__ __launch_bounds__(kThreads *GROUPS, 1) void matmul_tiles_kernel(MatmulArgs p,
+                                                                           int64_t tiles_m,
+                                                                           int64_t tiles_n) {
   constexpr int BM = 32 * MI, BN = 32 * NI, kRows = BM + BN;
   constexpr int kUnitBytes = kRows * 128;
   constexpr int kLoads = kRows / 32;                // a wave's loads of a unit, 8 rows each
   constexpr int kPart = (kLoads + MI - 1) / MI;     // of them after each row of products
-  constexpr int kScaleRows = (kRows + 255) & ~255;  // 64 rows to a load
-  __shared__ __align__(1024) uint8_t ring[2][kUnitBytes];
-  __shared__ __align__(1024) uint8_t scale_ring[2][kScaleRows * 16];
+  static_assert(kRows % 64 == 0 && GROUPS >= 1, "");
+  static_assert(GROUPS == 1 || MI * NI * 4096 <= 2 * kUnitBytes, "");  // the sums meet there
+  __shared__ __align__(1024) uint8_t rings[GROUPS][2][kUnitBytes];
+  __shared__ __align__(1024) uint8_t scale_rings[GROUPS][2][kRows * 16];
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) & 3;
   const int uw = __builtin_amdgcn_readfirstlane(wave);
+  const int group = GROUPS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  uint8_t(*ring)[kUnitBytes] = rings[group];
+  uint8_t(*scale_ring)[kRows * 16] = scale_rings[group];
   const int g = lane >> 4, i = lane & 15;
   const int wm = wave >> 1, wn = wave & 1;
   const int row_bytes = static_cast<int>(p.k / 2);
@@ -167,7 +176,10 @@ __global__ __launch_bounds__(kThreads, 1) void matmul_tiles_kernel(MatmulArgs p,
     off[q] = static_cast<uint32_t>(32 * q < BM ? min(row, last_m) : min(row - BM, last_n)) *
              row_bytes;
   }
+  // (Windows and units are counted within the group.)
+  auto window_of = [&](int win) { return GROUPS * win + group; };
   auto fetch = [&](int unit, int slot, int from, int to) {
+    if (GROUPS > 1) unit = 2 * window_of(unit >> 1) + (unit & 1);
     const uint32_t at = 16u * static_cast<uint32_t>(min(8 * unit + load_block, blocks - 1));
 #pragma unroll
     for (int q = 0; q < kLoads; ++q)
@@ -176,15 +188,12 @@ __global__ __launch_bounds__(kThreads, 1) void matmul_tiles_kernel(MatmulArgs p,
                        ring_at + slot * kUnitBytes + (4 * q + uw) * 1024);
   };
   auto fetch_scales = [&](int win) {
-    const uint8_t *wa = as + win * (p.m * 16), *wb = bs + win * (p.n * 16);
-#pragma unroll
-    for (int q = 0; q < kScaleRows / 256; ++q) {
-      const int row = 64 * (4 * q + uw);  // (BM is a multiple of 64; rows past kRows: any)
-      const bool of_a = row < BM;
-      const int from = of_a ? row : min(row - BM, BN - 64);
-      load_lds_async(of_a ? wa : wb, static_cast<uint32_t>(16 * (from + lane)),
-                     scale_at + (win & 1) * (kScaleRows * 16) + row * 16);
-    }
+    const int64_t w = GROUPS > 1 ? min(window_of(win), wins - 1) : win;
+    const uint8_t *wa = as + w * (p.m * 16), *wb = bs + w * (p.n * 16);
+    const int row = 64 * uw;  // (BM is a multiple of 64)
+    if (row < kRows)
+      load_lds_async(row < BM ? wa : wb, static_cast<uint32_t>(16 * ((row < BM ? row : row - BM) + lane)),
+                     scale_at + (win & 1) * (kRows * 16) + row * 16);
   };
 
   uint4 af[MI], bf[2][NI];
@@ -198,12 +207,18 @@ __global__ __launch_bounds__(kThreads, 1) void matmul_tiles_kernel(MatmulArgs p,
 #pragma unroll
     for (int t = 0; t < NI; ++t)
       sb[t] = *reinterpret_cast<const uint32_t *>(s + read_sb + 256 * t);
+    if (GROUPS > 1 && window_of(win) >= wins) {  // past K
+#pragma unroll
+      for (int t = 0; t < MI; ++t) sa[t] = 0;
+#pragma unroll
+      for (int t = 0; t < NI; ++t) sb[t] = 0;
+    }
   };
 
   fetch_scales(0);
   fetch(0, 0, 0, kLoads);
   fetch(1, 1, 0, kLoads);
-  const int units = 2 * wins;
+  const int rounds = (wins + GROUPS - 1) / GROUPS, units = 2 * rounds;
 #pragma unroll
   for (int x = 0; x < MI; ++x)
 #pragma unroll
@@ -231,17 +246,17 @@ __global__ __launch_bounds__(kThreads, 1) void matmul_tiles_kernel(MatmulArgs p,
       __builtin_amdgcn_sched_barrier(0);                                                       \
     }                                                                                          \
   }
-  for (int win = 0; win < wins; ++win) {
+  for (int win = 0; win < rounds; ++win) {
     int unit = 2 * win + 2;
     TKS_PHASE(0, 0, 1, false)
     unit_barrier();
-    if (win + 1 < wins) fetch_scales(win + 1);
+    if (win + 1 < rounds) fetch_scales(win + 1);
     TKS_PHASE(1, 1, 0, true)
     ++unit;
     TKS_PHASE(2, 1, 1, false)
     unit_barrier();
     TKS_PHASE(3, 0, 0, true)
-    if (win + 1 < wins)
+    if (win + 1 < rounds)
       get_scales(win + 1);
     else
       settle_sums();
@@ -249,8 +264,7 @@ __global__ __launch_bounds__(kThreads, 1) void matmul_tiles_kernel(MatmulArgs p,
 #undef TKS_PHASE
 
   T *out = static_cast<T *>(p.out) + m0 * p.o_rs + n0;
-#pragma unroll
-  for (int x = 0; x < MI; ++x) {
+  auto store = [&](int x, const mx_f4 *sums) {
     const int row = 16 * (MI * wm + x) + i;
     T *o = out + row * p.o_rs;
 #pragma unroll
@@ -260,20 +274,46 @@ __global__ __launch_bounds__(kThreads, 1) void matmul_tiles_kernel(MatmulArgs p,
         // Four columns are 8 bytes: lanes of neighbouring groups exchange halves of two column
         // tiles, so that each stores 16 (2048 x 11264: 42.9 -> 39.3 us).
         if (y & 1) continue;
-        const uint2 v = four16<T>(acc[x][y]), w = four16<T>(acc[x][y + 1]);
+        const uint2 v = four16<T>(sums[y]), w = four16<T>(sums[y + 1]);
         const uint4 both = swap_halves(v, w);
         const int at = 16 * (NI * wn + y + (g & 1)) + 8 * (g >> 1);
         if (row <= last_m && at <= last_n) st16(o + at, both);
       } else if constexpr (VEC) {
-        const mx_f4 v = acc[x][y];
+        const mx_f4 v = sums[y];
         if (row <= last_m && col <= last_n)
           st16(o + col, make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]),
                                    __float_as_uint(v[2]), __float_as_uint(v[3])));
       } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (row <= last_m && col + r <= last_n) o[col + r] = from_float<T>(acc[x][y][r]);
+          if (row <= last_m && col + r <= last_n) o[col + r] = from_float<T>(sums[y][r]);
       }
+    }
+  };
+  if constexpr (GROUPS == 1) {
+#pragma unroll
+    for (int x = 0; x < MI; ++x) store(x, acc[x]);
+  } else {
+    // (Every LDS read of the loop that matters is done, every load into LDS has come.) Group
+    // x adds up the x-th row of tiles of each wave of the four.
+    auto sums_of = [&](int from, int x, int y) {
+      return reinterpret_cast<mx_f4 *>(&rings[from][0][0]) + ((x * NI + y) * 4 + wave) * 64 + lane;
+    };
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < MI; ++x)
+#pragma unroll
+      for (int y = 0; y < NI; ++y) *sums_of(group, x, y) = acc[x][y];
+    __syncthreads();
+    for (int x = group; x < MI; x += GROUPS) {
+      mx_f4 sums[NI];
+#pragma unroll
+      for (int y = 0; y < NI; ++y) {
+        sums[y] = *sums_of(0, x, y);
+#pragma unroll
+        for (int from = 1; from < GROUPS; ++from) sums[y] += *sums_of(from, x, y);
+      }
+      store(x, sums);
     }
   }
 }
@@ -346,7 +386,7 @@ __global__ __launch_bounds__(kThreads) void quantize_windows_kernel(
   }
 }
 
-template <typename T, int MI, int NI>
+template <typename T, int MI, int NI, int GROUPS = 1>
 int32_t launch_tiles(const MatmulArgs &p, hipStream_t s) {
   const int64_t tm = ceil_div(p.m, 32 * MI), tn = ceil_div(p.n, 32 * NI);
   if (tm > 0x7fffffff / tn) return TKS_ERR_VALUE;
@@ -354,9 +394,9 @@ int32_t launch_tiles(const MatmulArgs &p, hipStream_t s) {
   // (Whole 16-byte pieces of a row: eight 16-bit columns, four fp32.)
   const bool vec = p.n * sizeof(T) % 16 == 0 && p.o_rs * sizeof(T) % 16 == 0 && aligned16(p.out);
   if (vec)
-    matmul_tiles_kernel<T, MI, NI, true><<<grid, kThreads, 0, s>>>(p, tm, tn);
+    matmul_tiles_kernel<T, MI, NI, GROUPS, true><<<grid, kThreads * GROUPS, 0, s>>>(p, tm, tn);
   else
-    matmul_tiles_kernel<T, MI, NI, false><<<grid, kThreads, 0, s>>>(p, tm, tn);
+    matmul_tiles_kernel<T, MI, NI, GROUPS, false><<<grid, kThreads * GROUPS, 0, s>>>(p, tm, tn);
   return check_launch();
 }
 
@@ -368,10 +408,19 @@ int32_t launch_tiles(const MatmulArgs &p, hipStream_t s) {
 //   300 x 11264 x 2048  (264; 440 of 64 x 128)      12.4, 10.0, 10.4
 //   777 x 2048 x 5632   (112; 208)                  16.1, 13.1, 12.6
 //   512 x 2048 x 2048   (64; 128)                   8.3, 6.6, 5.7
+// With no more tiles of 64 x 64 than CUs a workgroup waits for its loads most of the time, and
+// four groups of waves have four times as many on the way. us of a projection, its rows'
+// quantisation included, with one group and with four:
+//   128 x 2048 x 5632 (64 tiles) 16.4, 13.2     128 x 8192 x 4096 (256) 14.9, 12.8
+//   256 x 4096 x 11008 (256)     32.3, 24.9     128 x 2048 x 2048 (64)  9.7, 9.0
+//   777 x 2048 x 5632 (416)      20.6, 24.2     512 x 2560 x 2048 (320) 11.0, 13.7
+constexpr int64_t kFewTiles = 256;
 template <typename T>
 int32_t launch(const MatmulArgs &p, hipStream_t s) {
   if (ceil_div(p.m, 128) * ceil_div(p.n, 128) >= 512) return launch_tiles<T, 4, 4>(p, s);
   if (ceil_div(p.m, 64) * ceil_div(p.n, 128) >= 256) return launch_tiles<T, 2, 4>(p, s);
+  if (ceil_div(p.m, 64) * ceil_div(p.n, 64) <= kFewTiles && windows(p.k) >= 4)
+    return launch_tiles<T, 2, 2, 4>(p, s);
   return launch_tiles<T, 2, 2>(p, s);
 }
 

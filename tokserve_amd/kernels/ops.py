@@ -568,8 +568,8 @@ def mxfp4_linear(
 ) -> torch.Tensor:
     """A projection with MXFP4 weights (N, K): inputs (..., K) -> (..., N) in their dtype.
 
-    The rows are quantized as mxfp4_quantize does and multiplied as mxfp4_matmul does; the
-    results are those of the two calls. `workspace` as there, of mxfp4_linear_workspace_bytes.
+    The rows are quantized as mxfp4_quantize does and multiplied as mxfp4_matmul does;
+    the results are the two calls' up to the order of their fp32 sums. `workspace` as there, of mxfp4_linear_workspace_bytes.
     """
 
     device = require_hip("mxfp4_linear", inputs)
