@@ -205,6 +205,24 @@ def test_decode_of_long_sequences(device, dtype) -> None:
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("block_size,pages,bound", [(16, 600, 9000), (48, 0, 9000), (5, 2000, 9000),
+                                                    (100, 0, 2100), (32, 0, 12288), (16, 0, 2048)])
+def test_decode_of_long_splits(device, dtype, block_size, pages, bound) -> None:
+    """Splits of thousands of keys (a wave's tiles pass one look-up of pages), and the bound's
+    own choice, of every kind of block."""
+
+    lengths = [min(n, bound) for n in (9000, 4096, 4097, 2047, 31, 0)]
+    pool = Pool(lengths, 1, 64, block_size, device, seed=bound + block_size,
+                extra_width=-(-bound // block_size) - -(-max(lengths) // block_size))
+    query = torch.randn(6, 3, 64, generator=torch.Generator().manual_seed(2)).to(dtype)
+    out = ops.paged_attention_decode(query.to(device), pool.key, pool.value, pool.block_tables,
+                                     pool.lens, layer_index=0, max_seq_len=bound,
+                                     pages_per_split=pages, **pool.scales)
+    for b in range(6):
+        _check_attention(out[b:b + 1], query[b:b + 1], *pool.rows[b])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_decode_of_extreme_values(device, dtype) -> None:
     """Scores far apart (a reference that moves late), a zero query, a negative scale, and
     NaN or infinite inputs in one sequence, which stay in it."""

@@ -1187,6 +1187,39 @@ extern "C" int32_t tks_rope_append_paged_decode_fp8_rows(
 
 namespace {
 
+// Key splits of a decode over MXFP4 pools. A workgroup is through 128 keys in half a
+// microsecond, whatever it waits for, so the merge (a launch, 3 us) pays later than over the
+// other pools; never more splits than choose_pages_per_split has, whose workspace query serves
+// both. us of bf16 queries at 32 / 8 heads, Dh 128 and 32 / 4, Dh 64 (blocks of 16):
+//  * A bound below 2,048 keys: unsplit. One sequence of 512 keys 6.1 and 5.6 (two splits 8.5
+//    and 8.1), 16 of up to 1,152 8.4 and 7.3 (11.1 and 8.8).
+//  * Fewer than kFillItems pairs: 512 keys or what fills the CUs, up to 768 or an eighth of
+//    the bound. One sequence of 131,072 keys 31.6 (4,096-key splits; 54.8 at 768); one of up to 8,192
+//    10.3 and 9.7 at 512 keys, 11.9 and 11.2 at 256; 16 28.0 - 30 at any from 512 up.
+//  * Fewer than kSplitBelowItems: four keys per pair, or an eighth of the bound. Up to 8,192
+//    keys, log-uniform and from 4,096 up uniform: 256 pairs 23.3 and 44.5 at 1,024 keys, 25.4 and
+//    47.8 at 512, 32.5 and 47.2 at 2,048; 768 of Dh 64 42.5 and 86.1 at 4,096, 46.7 and 115.7 at 512.
+//  * Otherwise unsplit: 1,024 pairs 57.0 and 154, 62.0 and 188 at 1,024 keys.
+constexpr int64_t kMxSplitFrom = 2048;
+constexpr int64_t kMxMinSplit = 512, kMxFillSplit = 768, kMxSplitsOfBound = 8, kMxKeysPerItem = 4;
+int32_t choose_pages_mxfp4(int32_t num_seqs, int32_t num_kv_heads, int32_t block_size,
+                           int32_t max_seq_len, int32_t requested) {
+  const int32_t pps = choose_pages_per_split(num_seqs, num_kv_heads, block_size, max_seq_len,
+                                             requested, split_unit(block_size));
+  if (requested > 0) return pps;
+  const int64_t max_pages = ceil_div(max_seq_len > 0 ? max_seq_len : 1, block_size);
+  const int64_t items = static_cast<int64_t>(num_seqs) * num_kv_heads;
+  const int64_t bound = max_pages * block_size;
+  int64_t keys = bound;
+  if (bound >= kMxSplitFrom && items < kFillItems) {
+    const int64_t fill = ceil_div(max_pages, ceil_div(kFillItems, items)) * block_size;
+    keys = std::min(std::max(kMxMinSplit, fill), std::max(kMxFillSplit, bound / kMxSplitsOfBound));
+  } else if (bound >= kMxSplitFrom && items < kSplitBelowItems) {
+    keys = std::max(kMxKeysPerItem * items, bound / kMxSplitsOfBound);
+  }
+  return std::max(pps, static_cast<int32_t>(ceil_div(keys, block_size)));
+}
+
 int32_t decode_mxfp4_impl(const void *query, int64_t q_seq_stride, int64_t q_head_stride,
                           const void *key_cache, const void *value_cache, const void *k_scales,
                           const void *v_scales, int32_t num_layers, int64_t num_blocks,
@@ -1209,8 +1242,8 @@ int32_t decode_mxfp4_impl(const void *query, int64_t q_seq_stride, int64_t q_hea
   if (!query || !mx_pools_given(key_cache, value_cache, k_scales, v_scales) || !block_tables ||
       !seq_lens || !out)
     return TKS_ERR_VALUE;
-  const int32_t pps = choose_pages_per_split(num_seqs, num_kv_heads, block_size, max_seq_len,
-                                             pages_per_split, split_unit(block_size));
+  const int32_t pps =
+      choose_pages_mxfp4(num_seqs, num_kv_heads, block_size, max_seq_len, pages_per_split);
   const int32_t max_splits = split_count(max_seq_len, block_size, pps);
   if (max_splits > kMaxGridSplits) return TKS_ERR_VALUE;
   const Workspace w = carve(workspace, num_seqs, num_q_heads, max_splits, head_dim);
