@@ -525,12 +525,14 @@ int32_t tks_rope_append_paged_decode_mxfp4(
     int32_t pages_per_split, void *out, int64_t out_seq_stride, int64_t out_head_stride,
     void *workspace, int64_t workspace_bytes, int32_t dtype, tks_stream_t stream);
 
-/* Chunked-prefill attention: the pages the batch reads are decoded into the
- * workspace (a dense pool in `dtype` of ceil(max_seq_len / block_size) pages to a
- * sequence, values rounded once to it, and its identity block table; 16-byte aligned),
- * which tks_paged_attention_prefill then reads. */
-int64_t tks_paged_attention_prefill_mxfp4_workspace_bytes(int32_t num_seqs, int32_t num_kv_heads,
-                                                          int32_t head_dim, int32_t block_size,
+/* Chunked-prefill attention. Batches of many rows (a query token times a head of the group)
+ * per sequence and KV head need a workspace, 0 bytes otherwise: the pages they read are
+ * decoded into it (a dense pool in `dtype` of ceil(max_seq_len / block_size) pages to a
+ * sequence, values rounded once to it; 16-byte aligned). */
+int64_t tks_paged_attention_prefill_mxfp4_workspace_bytes(int32_t num_seqs, int64_t num_tokens,
+                                                          int32_t num_q_heads,
+                                                          int32_t num_kv_heads, int32_t head_dim,
+                                                          int32_t block_size,
                                                           int32_t max_seq_len, int32_t dtype);
 
 int32_t tks_paged_attention_prefill_mxfp4(

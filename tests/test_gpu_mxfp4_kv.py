@@ -318,6 +318,99 @@ def test_prefill(device, dtype, hq, hkv, dh, block_size) -> None:
         start += t
 
 
+# (Few rows; many: the waves of a workgroup share their keys; many of a sequence in 16 bits, Dh
+# 64 or 128 and blocks of a multiple of 16: over the decoded pages.)
+FORMS = [((6, 2, 96, 16), [(40, 30), (7, 100), (33, 0)]), ((8, 1, 32, 5), [(20, 300), (1, 0)]),
+         ((32, 8, 128, 16), [(113, 40 * k) for k in range(8)]),
+         ((64, 4, 32, 16), [(300, 70), (1, 9), (160, 0)]),
+         ((48, 3, 96, 24), [(590, 33), (12, 1100)]), ((64, 8, 64, 7), [(460, 129)]),
+         ((32, 2, 128, 48), [(900, 21)]), ((8, 1, 64, 16), [(260, 1090), (3, 40), (130, 0)]),
+         ((32, 4, 64, 32), [(129, 17), (150, 60)])]
+
+
+def _prefill(device, dtype, sizes, chunks, nan_at=None, short=None, **kw):
+    """One call, each sequence checked; behind the last query and between heads nothing is
+    written. nan_at: (sequence, key, head, block of V) that is NaN; short: a sequence of that
+    many keys, fewer than its queries."""
+
+    hq, hkv, dh, block_size = sizes
+    lengths = [t + p for t, p in chunks]
+    if short is not None:
+        lengths[-1] = short
+    pool = Pool(lengths, hkv, dh, block_size, device, seed=17, extra_width=3)
+    if nan_at is not None:
+        b, key, head, block = nan_at
+        at = pool.tables[b, key // block_size].item(), head, key % block_size, block
+        raw = pool.scales["v_scales"].view(torch.uint8)
+        raw[pool.layer][at] = 255
+    new = [t for t, _ in chunks]
+    cu = torch.tensor([0, *torch.tensor(new).cumsum(0).tolist()], dtype=torch.int32, device=device)
+    g = torch.Generator().manual_seed(5)
+    query = torch.randn(sum(new), hq, dh, generator=g).to(dtype)
+    canvas = torch.full((sum(new) + 3, hq, dh + 8), 7.0, dtype=dtype, device=device)
+    out = canvas[:sum(new), :, :dh]
+    got = ops.paged_attention_prefill(
+        query.to(device), pool.key, pool.value, pool.block_tables, pool.lens, cu, layer_index=0,
+        max_query_len=max(new), max_seq_len=max(lengths), out=out,
+        seq_order=ops.longest_first(lengths, device), **kw, **pool.scales)
+    assert got is out
+    assert bool((canvas[sum(new):] == 7).all()) and bool((canvas[:, :, dh:] == 7).all())
+    at = 0
+    for b, t in enumerate(new):
+        rows, x = out[at:at + t].cpu(), query[at:at + t]
+        at += t
+        none = max(0, t - lengths[b])  # rows of no keys
+        assert not rows[:none].any()
+        rows, x = rows[none:], x[none:]
+        if nan_at is not None and nan_at[0] == b:
+            _, key, head, block = nan_at
+            first = max(0, key - (lengths[b] - t))
+            hit = torch.zeros(rows.shape, dtype=torch.bool)
+            group = hq // hkv
+            hit[first:, head * group:(head + 1) * group, 32 * block:32 * block + 32] = True
+            assert torch.equal(rows.isnan(), hit)
+            # (The key's other blocks are as they were: the rest is checked against them.)
+            exact = mxfp4.attention(x, *pool.rows[b], kw.get("scale"))[0]
+            rows = torch.where(hit, exact.to(dtype), rows)
+        _check_attention(rows, x, *pool.rows[b], kw.get("scale"))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sizes,chunks", FORMS)
+def test_prefill_in_every_form(device, dtype, sizes, chunks) -> None:
+    _prefill(device, dtype, sizes, chunks)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sizes,chunks", FORMS)
+def test_prefill_reads_a_nan_block_only_where_it_is_seen(device, dtype, sizes, chunks) -> None:
+    """A value block of the first sequence that is NaN, in the middle of its queries."""
+
+    tokens, prior = chunks[0]
+    _prefill(device, dtype, sizes, chunks,
+             nan_at=(0, prior + tokens // 2, sizes[1] - 1, sizes[2] // 32 - 1))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sizes,chunks", [FORMS[0], FORMS[3], FORMS[7]])
+def test_prefill_of_more_queries_than_keys(device, dtype, sizes, chunks) -> None:
+    for short in (0, chunks[-1][0] // 2):
+        _prefill(device, dtype, sizes, chunks, short=short)
+
+
+@pytest.mark.parametrize("sizes,chunks", [FORMS[0], FORMS[3], FORMS[7]])
+@pytest.mark.parametrize("scale", [0.0, -0.3])
+def test_attention_of_any_scale(device, sizes, chunks, scale) -> None:
+    _prefill(device, torch.bfloat16, sizes, chunks, scale=scale)
+    pool = Pool([40, 3], sizes[1], sizes[2], 16, device, seed=4)
+    query = torch.randn(2, sizes[0], sizes[2], generator=torch.Generator().manual_seed(1))
+    out = ops.paged_attention_decode(query.to(device), pool.key, pool.value, pool.block_tables,
+                                     pool.lens, layer_index=0, max_seq_len=40, scale=scale,
+                                     **pool.scales)
+    for b in range(2):
+        _check_attention(out[b:b + 1], query[b:b + 1], *pool.rows[b], scale)
+
+
 # ------------------------------------------------------ the operators together
 
 

@@ -176,8 +176,14 @@ def test_c_entries_check_before_any_launch() -> None:
                         64, 64, None, 0, 0, None]
     assert decode(*args(keys=65)) == value and decode(*args(heads=17)) == value
     assert decode(*args(pages=1)) == space
-    assert library.tks_paged_attention_prefill_mxfp4_workspace_bytes(2, 1, 64, 16, 40, 0) == \
-        2 * (2 * 3 * 16 * 64 * 4) + 256
+    prefill = library.tks_paged_attention_prefill_mxfp4_workspace_bytes
+    assert prefill(2, 4, 4, 1, 64, 16, 40, 0) == 0  # (fp32: straight from the pools)
+    assert prefill(2, 511, 4, 1, 64, 16, 400, 2) == 0
+    assert prefill(2, 512, 4, 1, 64, 16, 400, 2) == \
+        2 * (2 * 25 * 16 * 64 * 2) + 256 + 1024  # K, V, the table, a byte per row
+    assert prefill(2, 512, 4, 1, 96, 16, 400, 2) == 0 == prefill(2, 512, 4, 1, 64, 24, 400, 2)
+    assert prefill(64, 1 << 20, 8, 8, 128, 16, 1 << 15, 2) == 0  # (too much of it)
+    assert prefill(2, 512, 4, 3, 64, 16, 400, 2) == -1
 
 
 def test_projections_on_the_cpu() -> None:

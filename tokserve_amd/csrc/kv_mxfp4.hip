@@ -169,12 +169,13 @@ __global__ __launch_bounds__(kThreads) void gather_mx_kernel(
 }
 
 // The pages that a batch reads, decoded into a dense pool of T: page (b, p) at block b * W + p
-// (W pages to a sequence, at most the table's width), with the identity table beside it.
+// (W pages to a sequence, at most the table's width), with the identity table and the V rows'
+// marks beside it.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void decode_mx_pages_kernel(
     MxPool kc, MxPool vc, const int32_t *__restrict__ bt, int32_t bt_stride,
     const int32_t *__restrict__ seq_lens, int32_t num_seqs, int32_t width, T *__restrict__ k_out,
-    T *__restrict__ v_out, int32_t *__restrict__ table_out) {
+    T *__restrict__ v_out, int32_t *__restrict__ table_out, uint8_t *__restrict__ marks) {
   const int64_t per_head = static_cast<int64_t>(kc.block_size) * kc.head_dim / 8;
   const int64_t per_page = per_head * kc.num_kv_heads;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
@@ -195,7 +196,56 @@ __global__ __launch_bounds__(kThreads) void decode_mx_pages_kernel(
   kc.values8(row + r, d, f);
   mx_store8<T, true>(k_out + dst, f);
   vc.values8(row + r, d, f);
+  const int nb = kc.head_dim / kMxBlock;
+  const uint8_t *vs = vc.scales + (row + r) * nb;
+  // (A NaN block would reach rows that do not see it, as 0 * NaN: mx_marks_kernel has them.)
+  if (vs[d / kMxBlock] == 255)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = 0.f;
   mx_store8<T, true>(v_out + dst, f);
+  if (d == 0) {
+    uint32_t mark = 0;
+    for (int j = 0; j < nb; ++j) mark |= static_cast<uint32_t>(vs[j] == 255) << j;
+    marks[dst / kc.head_dim] = static_cast<uint8_t>(mark);
+  }
+}
+
+// One workgroup per (sequence, KV head): the first key of each 32 dims that is NaN, and NaN to
+// those dims of the rows from its position on. A launch that mostly finds nothing, 2 us of it.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void mx_marks_kernel(MxPrefillArgs a,
+                                                            const uint8_t *__restrict__ marks,
+                                                            int32_t width) {
+  __shared__ int first[4];
+  const int b = blockIdx.y, kvh = blockIdx.x, BS = a.kc.block_size, G = a.group;
+  const int len = min(max(a.seq_lens[b], 0), a.key_cap);
+  if (threadIdx.x < 4) first[threadIdx.x] = INT32_MAX;
+  __syncthreads();
+  for (int key = 16 * static_cast<int>(threadIdx.x); key < len; key += 16 * kThreads) {
+    const int page = key / BS;
+    const int64_t at =
+        ((static_cast<int64_t>(b) * width + page) * a.kc.num_kv_heads + kvh) * BS + key - page * BS;
+    const uint4 v = *reinterpret_cast<const uint4 *>(marks + at);
+    // (Of a last page's rows past `len` too, which no row sees.)
+    if ((v.x | v.y | v.z | v.w) == 0) continue;
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    for (int e = 0; e < 16 && key + e < len; ++e)
+      for (int j = 0; j < 4; ++j)
+        if ((w[e >> 2] >> (8 * (e & 3) + j)) & 1) atomicMin(&first[j], key + e);
+  }
+  __syncthreads();
+  const int q0 = min(max(a.cu_q[b], 0), a.num_tokens);
+  const int q_len = min(a.cu_q[b + 1], a.num_tokens) - q0;
+  for (int j = 0; j < a.kc.head_dim / kMxBlock; ++j) {
+    if (first[j] == INT32_MAX) continue;
+    const int from = max(first[j] - (len - q_len), 0);  // the first token that sees it
+    const int64_t items = static_cast<int64_t>(q_len - from) * G * kMxBlock;
+    for (int64_t e = threadIdx.x; e < items; e += kThreads) {
+      const int64_t row = e / kMxBlock, t = q0 + from + row / G;
+      static_cast<T *>(a.out)[t * a.o_ts + (static_cast<int64_t>(kvh) * G + row % G) * a.o_hs +
+                              j * kMxBlock + e % kMxBlock] = from_float<T>(__builtin_nanf(""));
+    }
+  }
 }
 
 template <typename T>
@@ -262,12 +312,14 @@ MxScratch mx_carve_pages(void *ws, int32_t num_seqs, int32_t width, int32_t num_
   const int64_t pool =
       ceil_div(pages * num_kv_heads * block_size * head_dim * elem_bytes(dtype), 256) * 256;
   const int64_t table = ceil_div(pages * 4, 256) * 256;
+  const int64_t marks = ceil_div(pages * num_kv_heads * block_size, 256) * 256;
   char *base = static_cast<char *>(ws);
   MxScratch r;
   r.k = base;
   r.v = base ? base + pool : nullptr;
   r.table = base ? reinterpret_cast<int32_t *>(base + 2 * pool) : nullptr;
-  r.bytes = 2 * pool + table;
+  r.marks = base ? reinterpret_cast<uint8_t *>(base + 2 * pool + table) : nullptr;
+  r.bytes = 2 * pool + table + marks;
   return r;
 }
 
@@ -278,16 +330,26 @@ int32_t launch_decode_mx_pages(const MxPool &kc, const MxPool &vc, const int32_t
                         kc.block_size * (kc.head_dim / 8);
   if (ceil_div(items, kThreads) > 0x7fffffff) return TKS_ERR_VALUE;
   const unsigned grid = static_cast<unsigned>(ceil_div(items, kThreads));
-#define TKS_MX_PAGES(TYPE)                                                                    \
-  decode_mx_pages_kernel<TYPE><<<grid, kThreads, 0, s>>>(                                     \
-      kc, vc, bt, bt_stride, seq_lens, num_seqs, width, static_cast<TYPE *>(to.k),                   \
-      static_cast<TYPE *>(to.v), to.table)
-  switch (dtype) {
-    case TKS_FLOAT32: TKS_MX_PAGES(float); break;
-    case TKS_FLOAT16: TKS_MX_PAGES(_Float16); break;
-    default: TKS_MX_PAGES(bf16_t); break;
-  }
-#undef TKS_MX_PAGES
+  auto run = [&](auto zero) {
+    typedef decltype(zero) T;
+    decode_mx_pages_kernel<T><<<grid, kThreads, 0, s>>>(
+        kc, vc, bt, bt_stride, seq_lens, num_seqs, width, static_cast<T *>(to.k),
+        static_cast<T *>(to.v), to.table, to.marks);
+  };
+  if (dtype == TKS_FLOAT16)
+    run(_Float16());
+  else
+    run(bf16_t());
+  return check_launch();
+}
+
+int32_t launch_mx_marks(const MxPrefillArgs &a, const MxScratch &from, int32_t width,
+                        int32_t dtype, hipStream_t s) {
+  const dim3 grid(a.kc.num_kv_heads, a.num_seqs);
+  if (dtype == TKS_FLOAT16)
+    mx_marks_kernel<_Float16><<<grid, kThreads, 0, s>>>(a, from.marks, width);
+  else
+    mx_marks_kernel<bf16_t><<<grid, kThreads, 0, s>>>(a, from.marks, width);
   return check_launch();
 }
 

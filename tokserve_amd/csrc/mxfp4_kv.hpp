@@ -1,5 +1,5 @@
-// MXFP4 K/V pools as the kernels address them, and the scratch pool that a prefill decodes
-// the pages it reads into.
+// MXFP4 K/V pools as the kernels address them, and the scratch pool that a prefill of many rows
+// decodes the pages it reads into.
 #pragma once
 
 #include "mxfp4_common.hpp"
@@ -48,11 +48,13 @@ inline MxPool mx_pool(void *codes, void *scales, int64_t num_blocks, int32_t num
                 head_dim};
 }
 
-// Pages decoded for a prefill: pools of the query's dtype, num_seqs * width blocks, and the
-// identity block table.
+// Pages decoded for a prefill (16-bit types, blocks of a multiple of 16 tokens): pools of the
+// query's dtype, num_seqs * width blocks, the identity block table, and a byte per V row (in
+// the pools' order), bit j: its j-th block is NaN, zeros in the pool.
 struct MxScratch {
   void *k, *v;
   int32_t *table;
+  uint8_t *marks;
   int64_t bytes;
 };
 MxScratch mx_carve_pages(void *ws, int32_t num_seqs, int32_t width, int32_t num_kv_heads,
@@ -60,6 +62,10 @@ MxScratch mx_carve_pages(void *ws, int32_t num_seqs, int32_t width, int32_t num_
 int32_t launch_decode_mx_pages(const MxPool &kc, const MxPool &vc, const int32_t *bt,
                                int32_t bt_stride, const int32_t *seq_lens, int32_t num_seqs,
                                int32_t width, const MxScratch &to, int32_t dtype, hipStream_t s);
+struct MxPrefillArgs;
+// NaN to the outputs of the rows that see a marked block.
+int32_t launch_mx_marks(const MxPrefillArgs &a, const MxScratch &from, int32_t width,
+                        int32_t dtype, hipStream_t s);
 
 // Decode attention over MXFP4 pools (decode_mxfp4.hip).
 struct MxDecodeArgs {
@@ -81,5 +87,24 @@ struct MxDecodeArgs {
 };
 int32_t launch_decode_mxfp4(const MxDecodeArgs &a, int32_t dtype, int32_t num_seqs,
                             hipStream_t s);
+
+// Chunked prefill over them (prefill_mxfp4.hip).
+struct MxPrefillArgs {
+  const void *q;
+  int64_t q_ts, q_hs;
+  bool q_vec, o_vec;  // rows can be read and written 16 bytes at a time
+  MxPool kc, vc;
+  const int32_t *bt;
+  int32_t bt_stride;
+  const int32_t *seq_lens, *cu_q, *seq_order;
+  int32_t num_seqs, num_tokens, group;
+  float scale_log2;
+  int32_t key_cap;  // keys any sequence may have
+  int32_t tiles;    // of a sequence and KV head
+  void *out;
+  int64_t o_ts, o_hs;
+};
+int32_t launch_prefill_mxfp4(const MxPrefillArgs &a, int32_t max_query_len, int32_t dtype,
+                             hipStream_t s);
 
 }  // namespace tks

@@ -1344,17 +1344,48 @@ extern "C" int32_t tks_rope_append_paged_decode_mxfp4(
                            stream);
 }
 
+namespace {
+
+// Whether a prefill over MXFP4 pools decodes the pages it reads into a scratch pool of its type,
+// for the kernel of the 16-bit pools, which has two thirds to nine tenths of the other's time
+// where a (sequence, KV head) has enough rows to pay for the decoding. us so and straight from
+// the pools (prefill_mxfp4.hip), 32 heads: bf16, 8 KV heads of Dh 128, 16 x 512 tokens after up
+// to 2,048 keys 273 and 339 (2,048 rows), 16 x 256 after 4,096 240 and 269 (1,024), 16 x 128 160
+// and 147 (512), 64 x 64 381 and 259 (256); fp16 16 x 256 243 and 377, 64 x 64 384 and 364; bf16, 4
+// KV heads of Dh 64, 16 x 256 142 and 152 (2,048), 16 x 128 96 and 83 (1,024), 64 x 64 162 and 148
+// (512). Not for more than kMaxDecoded bytes of it.
+constexpr int64_t kDecodedRows = 1024;
+constexpr int64_t kMaxDecoded = int64_t{1} << 30;
+bool decodes_pages(int32_t num_seqs, int64_t num_tokens, int32_t num_q_heads,
+                   int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t max_seq_len,
+                   int32_t dtype, MxScratch *sp) {
+  const int32_t group = num_q_heads / num_kv_heads;
+  const int64_t width = ceil_div(std::max(max_seq_len, 1), block_size);
+  if (dtype == TKS_FLOAT32 || num_tokens * group < kDecodedRows * num_seqs || num_seqs > 65535 ||
+      num_seqs * width > INT32_MAX || width * block_size > INT32_MAX - 64 ||
+      !prefill_mfma_supported(dtype, head_dim, group, static_cast<int32_t>(width * block_size),
+                              block_size, num_seqs * width, num_kv_heads))
+    return false;
+  *sp = mx_carve_pages(nullptr, num_seqs, static_cast<int32_t>(width), num_kv_heads, block_size,
+                       head_dim, dtype);
+  return sp->bytes <= kMaxDecoded;
+}
+
+}  // namespace
+
 extern "C" int64_t tks_paged_attention_prefill_mxfp4_workspace_bytes(
-    int32_t num_seqs, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
-    int32_t max_seq_len, int32_t dtype) {
-  if (!valid_dtype(dtype) || num_seqs < 0 || num_kv_heads <= 0 || head_dim <= 0 ||
+    int32_t num_seqs, int64_t num_tokens, int32_t num_q_heads, int32_t num_kv_heads,
+    int32_t head_dim, int32_t block_size, int32_t max_seq_len, int32_t dtype) {
+  if (!valid_dtype(dtype) || num_seqs < 0 || num_tokens < 0 || num_tokens > 0x7fffffff ||
+      num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads != 0 || head_dim <= 0 ||
       block_size <= 0 || max_seq_len < 0)
     return -1;
-  return mx_carve_pages(nullptr, num_seqs,
-                        static_cast<int32_t>(ceil_div(std::max(max_seq_len, 1), block_size)),
-                        num_kv_heads,
-                        block_size, head_dim, dtype)
-      .bytes;
+  MxScratch sp{};
+  return num_seqs > 0 && num_tokens > 0 &&
+                 decodes_pages(num_seqs, num_tokens, num_q_heads, num_kv_heads, head_dim,
+                               block_size, max_seq_len, dtype, &sp)
+             ? sp.bytes
+             : 0;
 }
 
 extern "C" int32_t tks_paged_attention_prefill_mxfp4(
@@ -1377,28 +1408,55 @@ extern "C" int32_t tks_paged_attention_prefill_mxfp4(
   if (num_seqs == 0 || num_tokens == 0) return TKS_OK;
   if (num_tokens > 0x7fffffff || ceil_div(max_seq_len, block_size) > block_table_stride)
     return TKS_ERR_VALUE;
-  // (Queries of no keys: one page, of which nothing is read.)
-  const int32_t width = static_cast<int32_t>(ceil_div(std::max(max_seq_len, 1), block_size));
-  if (static_cast<int64_t>(num_seqs) * width > INT32_MAX) return TKS_ERR_VALUE;
   if (!query || !mx_pools_given(key_cache, value_cache, k_scales, v_scales) || !block_tables ||
       !seq_lens || !cu_seqlens_q || !out)
     return TKS_ERR_VALUE;
-  const MxScratch sp = mx_carve_pages(workspace, num_seqs, width, num_kv_heads, block_size,
-                                      head_dim, dtype);
+  // (Queries of no keys: one page, of which nothing is read.)
+  const int64_t width = ceil_div(std::max(max_seq_len, 1), block_size);
+  const int elem = elem_bytes(dtype);
+  MxPrefillArgs a{};
+  a.q = query;
+  a.q_ts = q_token_stride;
+  a.q_hs = q_head_stride;
+  a.q_vec = aligned16(query) && q_token_stride * elem % 16 == 0 && q_head_stride * elem % 16 == 0;
+  a.o_vec = aligned16(out) && out_token_stride * elem % 16 == 0 && out_head_stride * elem % 16 == 0;
+  a.kc = mx_pool(const_cast<void *>(key_cache), const_cast<void *>(k_scales), num_blocks,
+                 num_kv_heads, block_size, head_dim, layer_index);
+  a.vc = mx_pool(const_cast<void *>(value_cache), const_cast<void *>(v_scales), num_blocks,
+                 num_kv_heads, block_size, head_dim, layer_index);
+  a.bt = block_tables;
+  a.bt_stride = block_table_stride;
+  a.seq_lens = seq_lens;
+  a.cu_q = cu_seqlens_q;
+  a.seq_order = seq_order;
+  a.num_seqs = num_seqs;
+  a.num_tokens = static_cast<int32_t>(num_tokens);
+  a.group = num_q_heads / num_kv_heads;
+  a.scale_log2 = scale * kLog2e;
+  a.key_cap = static_cast<int32_t>(
+      std::min<int64_t>(std::min<int64_t>(block_table_stride, width) * block_size, INT32_MAX - 64));
+  a.out = out;
+  a.o_ts = out_token_stride;
+  a.o_hs = out_head_stride;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  MxScratch sp{};
+  if (!decodes_pages(num_seqs, num_tokens, num_q_heads, num_kv_heads, head_dim, block_size,
+                     max_seq_len, dtype, &sp))
+    return launch_prefill_mxfp4(a, max_query_len, dtype, s);
   if (workspace == nullptr || workspace_bytes < sp.bytes || !aligned16(workspace))
     return TKS_ERR_WORKSPACE;
-  const MxPool kc = mx_pool(const_cast<void *>(key_cache), const_cast<void *>(k_scales),
-                            num_blocks, num_kv_heads, block_size, head_dim, layer_index);
-  const MxPool vc = mx_pool(const_cast<void *>(value_cache), const_cast<void *>(v_scales),
-                            num_blocks, num_kv_heads, block_size, head_dim, layer_index);
-  const int32_t st =
-      launch_decode_mx_pages(kc, vc, block_tables, block_table_stride, seq_lens, num_seqs, width,
-                             sp, dtype, static_cast<hipStream_t>(stream));
+  // (The 16-bit pools' kernel reads whole rows 16 bytes at a time, and takes positive scales.)
+  if (!a.q_vec || !(a.scale_log2 > 0.f && a.scale_log2 < INFINITY))
+    return launch_prefill_mxfp4(a, max_query_len, dtype, s);
+  const int32_t w = static_cast<int32_t>(width);
+  sp = mx_carve_pages(workspace, num_seqs, w, num_kv_heads, block_size, head_dim, dtype);
+  int32_t st = launch_decode_mx_pages(a.kc, a.vc, block_tables, block_table_stride, seq_lens,
+                                      num_seqs, w, sp, dtype, s);
   if (st != TKS_OK) return st;
-  return prefill_impl(query, q_token_stride, q_head_stride, sp.k, sp.v, 1,
-                      static_cast<int64_t>(num_seqs) * width, num_kv_heads,
-                      block_size, head_dim, 0, sp.table, width, seq_lens,
-                      cu_seqlens_q, seq_order, num_seqs, num_tokens, num_q_heads, max_query_len,
-                      max_seq_len, scale, out, out_token_stride, out_head_stride, false, nullptr,
-                      0, 1.f, 1.f, dtype, stream);
+  st = prefill_impl(query, q_token_stride, q_head_stride, sp.k, sp.v, 1,
+                    static_cast<int64_t>(num_seqs) * w, num_kv_heads, block_size, head_dim, 0,
+                    sp.table, w, seq_lens, cu_seqlens_q, seq_order, num_seqs, num_tokens,
+                    num_q_heads, max_query_len, max_seq_len, scale, out, out_token_stride,
+                    out_head_stride, false, nullptr, 0, 1.f, 1.f, dtype, stream);
+  return st != TKS_OK ? st : launch_mx_marks(a, sp, w, dtype, s);
 }

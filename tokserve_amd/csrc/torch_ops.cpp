@@ -258,8 +258,9 @@ void paged_attention_prefill(const Tensor &query, const Tensor &key_cache,
   int32_t status;
   if (mxfp4(kc)) {
     const Tensor ws = scratch(l.tks_paged_attention_prefill_mxfp4_workspace_bytes(
-                                  i32(seq_lens.size(0)), i32(kc.size(2)), head_dim(kc),
-                                  i32(kc.size(3)), i32(max_seq_len), code(query)),
+                                  i32(seq_lens.size(0)), query.size(0), i32(query.size(1)),
+                                  i32(kc.size(2)), head_dim(kc), i32(kc.size(3)),
+                                  i32(max_seq_len), code(query)),
                               query, "MXFP4 prefill");
     status = call(l.tks_paged_attention_prefill_mxfp4,
                   std::make_tuple(ptr(k_scales), ptr(v_scales)),

@@ -242,7 +242,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ),
     "tks_paged_attention_prefill_mxfp4_workspace_bytes": (
         _i64,
-        [_i32, _i32, _i32, _i32, _i32, _i32],
+        [_i32, _i64, _i32, _i32, _i32, _i32, _i32, _i32],
     ),
     "tks_paged_attention_prefill_mxfp4": (
         _i32,

@@ -443,7 +443,7 @@ def paged_attention_prefill(
     e.g. longest_first of seq_lens) is the order in which sequences reach
     workgroups; results do not depend on it. fp8 pools are decoded with
     (k_scale, v_scale), or per row with k_scales / v_scales; MXFP4 pools with
-    k_scales / v_scales, their values rounded to the query's dtype.
+    k_scales / v_scales.
     """
 
     require_hip(
