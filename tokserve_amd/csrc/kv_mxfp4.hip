@@ -11,6 +11,8 @@
 
 #include <algorithm>
 
+#include <type_traits>
+
 namespace tks {
 namespace {
 
@@ -170,43 +172,39 @@ __global__ __launch_bounds__(kThreads) void gather_mx_kernel(
 
 // The pages that a batch reads, decoded into a dense pool of T: page (b, p) at block b * W + p
 // (W pages to a sequence, at most the table's width), with the identity table and the V rows'
-// marks beside it.
-template <typename T>
+// marks beside it. A workgroup decodes a page, eight values a thread at a time.
+template <typename T, int NB>
 __global__ __launch_bounds__(kThreads) void decode_mx_pages_kernel(
     MxPool kc, MxPool vc, const int32_t *__restrict__ bt, int32_t bt_stride,
-    const int32_t *__restrict__ seq_lens, int32_t num_seqs, int32_t width, T *__restrict__ k_out,
+    const int32_t *__restrict__ seq_lens, int32_t width, T *__restrict__ k_out,
     T *__restrict__ v_out, int32_t *__restrict__ table_out, uint8_t *__restrict__ marks) {
-  const int64_t per_head = static_cast<int64_t>(kc.block_size) * kc.head_dim / 8;
-  const int64_t per_page = per_head * kc.num_kv_heads;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const int64_t at = item / per_page;  // b * W + p
-  if (at >= static_cast<int64_t>(num_seqs) * width) return;
-  const int b = static_cast<int>(at / width);
-  const int p = static_cast<int>(at - static_cast<int64_t>(b) * width);
-  const int64_t rem = item - at * per_page;
-  if (rem == 0) table_out[at] = static_cast<int32_t>(at);
-  const int64_t len = max(seq_lens[b], 0);
-  if (p * static_cast<int64_t>(kc.block_size) >= len) return;
+  constexpr int kEights = 4 * NB;  // of a row
+  const int at = blockIdx.x, b = at / width, p = at - b * width;
+  if (threadIdx.x == 0) table_out[at] = at;
+  if (p * static_cast<int64_t>(kc.block_size) >= seq_lens[b]) return;
   const int64_t block = block_of(bt + static_cast<int64_t>(b) * bt_stride, p, kc.num_blocks);
-  const int64_t row = (kc.layer_base + block * kc.num_kv_heads) * kc.block_size;
-  const int64_t r = rem * 8 / kc.head_dim;
-  const int d = static_cast<int>(rem * 8 - r * kc.head_dim);
-  const int64_t dst = (at * per_page + rem) * 8;
-  float f[8];
-  kc.values8(row + r, d, f);
-  mx_store8<T, true>(k_out + dst, f);
-  vc.values8(row + r, d, f);
-  const int nb = kc.head_dim / kMxBlock;
-  const uint8_t *vs = vc.scales + (row + r) * nb;
-  // (A NaN block would reach rows that do not see it, as 0 * NaN: mx_marks_kernel has them.)
-  if (vs[d / kMxBlock] == 255)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = 0.f;
-  mx_store8<T, true>(v_out + dst, f);
-  if (d == 0) {
+  const int64_t from = (kc.layer_base + block * kc.num_kv_heads) * kc.block_size;
+  const int rows = kc.num_kv_heads * kc.block_size;
+  const int64_t to = static_cast<int64_t>(at) * rows;
+  const uint32_t *k_codes = reinterpret_cast<const uint32_t *>(kc.codes + from * (16 * NB));
+  const uint32_t *v_codes = reinterpret_cast<const uint32_t *>(vc.codes + from * (16 * NB));
+  const uint8_t *k_scales = kc.scales + from * NB, *v_scales = vc.scales + from * NB;
+  T *k_to = k_out + to * (32 * NB), *v_to = v_out + to * (32 * NB);
+#pragma unroll 4
+  for (int e = threadIdx.x; e < rows * kEights; e += kThreads) {
+    float f[8];
+    mx_values8(k_codes[e], mx_scale(k_scales[e >> 2]), f);
+    mx_store8<T, true>(k_to + 8 * e, f);
+    const int r = e / kEights;
     uint32_t mark = 0;
-    for (int j = 0; j < nb; ++j) mark |= static_cast<uint32_t>(vs[j] == 255) << j;
-    marks[dst / kc.head_dim] = static_cast<uint8_t>(mark);
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      mark |= static_cast<uint32_t>(v_scales[r * NB + j] == 255) << j;
+    // (A NaN block would reach rows that do not see it, as 0 * NaN: mx_marks_kernel has them.)
+    const bool nan = (mark >> (e / 4 % NB)) & 1;
+    mx_values8(nan ? 0 : v_codes[e], mx_scale(nan ? 127 : v_scales[e >> 2]), f);
+    mx_store8<T, true>(v_to + 8 * e, f);
+    if (e % kEights == 0) marks[to + r] = static_cast<uint8_t>(mark);
   }
 }
 
@@ -326,20 +324,23 @@ MxScratch mx_carve_pages(void *ws, int32_t num_seqs, int32_t width, int32_t num_
 int32_t launch_decode_mx_pages(const MxPool &kc, const MxPool &vc, const int32_t *bt,
                                int32_t bt_stride, const int32_t *seq_lens, int32_t num_seqs,
                                int32_t width, const MxScratch &to, int32_t dtype, hipStream_t s) {
-  const int64_t items = static_cast<int64_t>(num_seqs) * width * kc.num_kv_heads *
-                        kc.block_size * (kc.head_dim / 8);
-  if (ceil_div(items, kThreads) > 0x7fffffff) return TKS_ERR_VALUE;
-  const unsigned grid = static_cast<unsigned>(ceil_div(items, kThreads));
-  auto run = [&](auto zero) {
+  const unsigned grid = static_cast<unsigned>(num_seqs) * static_cast<unsigned>(width);
+  auto run = [&](auto zero, auto nb) {
     typedef decltype(zero) T;
-    decode_mx_pages_kernel<T><<<grid, kThreads, 0, s>>>(
-        kc, vc, bt, bt_stride, seq_lens, num_seqs, width, static_cast<T *>(to.k),
-        static_cast<T *>(to.v), to.table, to.marks);
+    decode_mx_pages_kernel<T, decltype(nb)::value><<<grid, kThreads, 0, s>>>(
+        kc, vc, bt, bt_stride, seq_lens, width, static_cast<T *>(to.k), static_cast<T *>(to.v),
+        to.table, to.marks);
+  };
+  auto run_dh = [&](auto zero) {
+    if (kc.head_dim == 64)
+      run(zero, std::integral_constant<int, 2>());
+    else
+      run(zero, std::integral_constant<int, 4>());
   };
   if (dtype == TKS_FLOAT16)
-    run(_Float16());
+    run_dh(_Float16());
   else
-    run(bf16_t());
+    run_dh(bf16_t());
   return check_launch();
 }
 

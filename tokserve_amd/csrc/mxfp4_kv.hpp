@@ -48,7 +48,7 @@ inline MxPool mx_pool(void *codes, void *scales, int64_t num_blocks, int32_t num
                 head_dim};
 }
 
-// Pages decoded for a prefill (16-bit types, blocks of a multiple of 16 tokens): pools of the
+// Pages decoded for a prefill (16-bit types, Dh 64 or 128, blocks of a multiple of 16 tokens): pools of the
 // query's dtype, num_seqs * width blocks, the identity block table, and a byte per V row (in
 // the pools' order), bit j: its j-th block is NaN, zeros in the pool.
 struct MxScratch {
