@@ -318,14 +318,15 @@ def test_prefill(device, dtype, hq, hkv, dh, block_size) -> None:
         start += t
 
 
-# (Few rows; many: the waves of a workgroup share their keys; many of a sequence in 16 bits, Dh
-# 64 or 128 and blocks of a multiple of 16: over the decoded pages.)
+# (Few rows; many: the waves of a workgroup share their keys; many of a sequence and many keys
+# in 16 bits, Dh 64 or 128 and blocks of a multiple of 16: over the decoded pages.)
 FORMS = [((6, 2, 96, 16), [(40, 30), (7, 100), (33, 0)]), ((8, 1, 32, 5), [(20, 300), (1, 0)]),
          ((32, 8, 128, 16), [(113, 40 * k) for k in range(8)]),
          ((64, 4, 32, 16), [(300, 70), (1, 9), (160, 0)]),
          ((48, 3, 96, 24), [(590, 33), (12, 1100)]), ((64, 8, 64, 7), [(460, 129)]),
          ((32, 2, 128, 48), [(900, 21)]), ((8, 1, 64, 16), [(260, 1090), (3, 40), (130, 0)]),
-         ((32, 4, 64, 32), [(129, 17), (150, 60)])]
+         ((32, 4, 64, 32), [(129, 17), (150, 60)]), ((16, 1, 64, 32), [(300, 700)]),
+         ((8, 1, 128, 16), [(260, 1090), (3, 40), (130, 0)])]
 
 
 def _prefill(device, dtype, sizes, chunks, nan_at=None, short=None, **kw):
@@ -392,13 +393,13 @@ def test_prefill_reads_a_nan_block_only_where_it_is_seen(device, dtype, sizes, c
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("sizes,chunks", [FORMS[0], FORMS[3], FORMS[7]])
+@pytest.mark.parametrize("sizes,chunks", [FORMS[0], FORMS[3], FORMS[7], FORMS[10]])
 def test_prefill_of_more_queries_than_keys(device, dtype, sizes, chunks) -> None:
     for short in (0, chunks[-1][0] // 2):
         _prefill(device, dtype, sizes, chunks, short=short)
 
 
-@pytest.mark.parametrize("sizes,chunks", [FORMS[0], FORMS[3], FORMS[7]])
+@pytest.mark.parametrize("sizes,chunks", [FORMS[0], FORMS[3], FORMS[7], FORMS[10]])
 @pytest.mark.parametrize("scale", [0.0, -0.3])
 def test_attention_of_any_scale(device, sizes, chunks, scale) -> None:
     _prefill(device, torch.bfloat16, sizes, chunks, scale=scale)

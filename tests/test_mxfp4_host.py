@@ -178,12 +178,13 @@ def test_c_entries_check_before_any_launch() -> None:
     assert decode(*args(pages=1)) == space
     prefill = library.tks_paged_attention_prefill_mxfp4_workspace_bytes
     assert prefill(2, 4, 4, 1, 64, 16, 40, 0) == 0  # (fp32: straight from the pools)
-    assert prefill(2, 511, 4, 1, 64, 16, 400, 2) == 0
-    assert prefill(2, 512, 4, 1, 64, 16, 400, 2) == \
-        2 * (2 * 25 * 16 * 64 * 2) + 256 + 1024  # K, V, the table, a byte per row
-    assert prefill(2, 512, 4, 1, 96, 16, 400, 2) == 0 == prefill(2, 512, 4, 1, 64, 24, 400, 2)
+    assert prefill(2, 511, 4, 1, 128, 16, 512, 2) == 0 == prefill(2, 512, 4, 1, 128, 16, 511, 2)
+    assert prefill(2, 512, 4, 1, 128, 16, 512, 2) == \
+        2 * (2 * 32 * 16 * 128 * 2) + 256 + 1024  # K, V, the table, a byte per row
+    assert prefill(2, 512, 4, 1, 96, 16, 512, 2) == 0 == prefill(2, 512, 4, 1, 128, 24, 512, 2)
+    assert prefill(2, 512, 4, 1, 64, 16, 512, 2) == 0 < prefill(2, 2048, 4, 1, 64, 16, 1024, 2)
     assert prefill(64, 1 << 20, 8, 8, 128, 16, 1 << 15, 2) == 0  # (too much of it)
-    assert prefill(2, 512, 4, 3, 64, 16, 400, 2) == -1
+    assert prefill(2, 512, 4, 3, 128, 16, 512, 2) == -1
 
 
 def test_projections_on_the_cpu() -> None:

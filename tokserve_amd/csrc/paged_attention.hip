@@ -1347,22 +1347,26 @@ extern "C" int32_t tks_rope_append_paged_decode_mxfp4(
 namespace {
 
 // Whether a prefill over MXFP4 pools decodes the pages it reads into a scratch pool of its type,
-// for the kernel of the 16-bit pools, which has two thirds to nine tenths of the other's time
-// where a (sequence, KV head) has enough rows to pay for the decoding. us so and straight from
-// the pools (prefill_mxfp4.hip), 32 heads: bf16, 8 KV heads of Dh 128, 16 x 512 tokens after up
-// to 2,048 keys 273 and 339 (2,048 rows), 16 x 256 after 4,096 240 and 269 (1,024), 16 x 128 160
-// and 147 (512), 64 x 64 381 and 259 (256); fp16 16 x 256 243 and 377, 64 x 64 384 and 364; bf16, 4
-// KV heads of Dh 64, 16 x 256 142 and 152 (2,048), 16 x 128 96 and 83 (1,024), 64 x 64 162 and 148
-// (512). Not for more than kMaxDecoded bytes of it.
+// for the kernel of the 16-bit pools: two launches more, and nine tenths to two thirds of the
+// time where a (sequence, KV head) has enough rows, and rows times keys, to pay for them. us so
+// and straight from the pools (prefill_mxfp4.hip), 32 heads: bf16, 8 KV heads of Dh 128, 16 x 512
+// tokens after up to 2,048 keys 278 and 335 (2,048 rows), 16 x 256 after 4,096 240 and 269 (1,024),
+// 4 x 256 after none 23 and 22, 16 x 128 after 4,096 160 and 147 (512), 64 x 64 381 and 259 (256);
+// fp16 16 x 256 243 and 377, 64 x 64 384 and 364; bf16, 4 KV heads of Dh 64, 16 x 512 after up to
+// 2,048 162 and 180 (4,096 rows, 10M), 8 x 512 after none 49 and 40 (2M), 4 x 100-300 after up to 300
+// 22 and 19 (1M). Not for more than kMaxDecoded bytes of it.
 constexpr int64_t kDecodedRows = 1024;
+constexpr int64_t kDecodedWork = int64_t{1} << 19, kDecodedWork64 = int64_t{1} << 22;
 constexpr int64_t kMaxDecoded = int64_t{1} << 30;
 bool decodes_pages(int32_t num_seqs, int64_t num_tokens, int32_t num_q_heads,
                    int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t max_seq_len,
                    int32_t dtype, MxScratch *sp) {
   const int32_t group = num_q_heads / num_kv_heads;
   const int64_t width = ceil_div(std::max(max_seq_len, 1), block_size);
-  if (dtype == TKS_FLOAT32 || num_tokens * group < kDecodedRows * num_seqs || num_seqs > 65535 ||
-      num_seqs * width > INT32_MAX || width * block_size > INT32_MAX - 64 ||
+  const int64_t rows = num_tokens * group / num_seqs;
+  if (dtype == TKS_FLOAT32 || rows < kDecodedRows ||
+      rows * max_seq_len < (head_dim == 64 ? kDecodedWork64 : kDecodedWork) ||
+      num_seqs > 65535 || num_seqs * width > INT32_MAX || width * block_size > INT32_MAX - 64 ||
       !prefill_mfma_supported(dtype, head_dim, group, static_cast<int32_t>(width * block_size),
                               block_size, num_seqs * width, num_kv_heads))
     return false;

@@ -16,7 +16,7 @@
 // us of each (apart, shared), kv heads 8 of Dh 128 under 32 heads, 4,096 earlier keys: bf16 4 x
 // 128 tokens 44, 109; 16 x 64 85, 115; 16 x 128 163, 147; 512 earlier keys: 4 x 128 22, 26; 16 x
 // 64 35, 27; fp32 5 x 1-333 tokens, Dh 64, to 1,024 earlier: 23, 32 (over decoded fp32 pages, as
-// before these: 61); fp32 16 x 512, Dh 128, to 2,048 earlier: 642, 556 (1,590); bf16 4 x 200-400,
+// before these: 61); fp32 16 x 512, Dh 128, to 2,048 earlier: 642, 594 (1,590); bf16 4 x 200-400,
 // Dh 96, to 1,024 earlier: 76, 45 (3,910: nothing but a plain kernel takes such pages).
 #include "mxfp4_attention.hpp"
 
@@ -231,7 +231,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_mx_shared_kernel(MxPrefil
       unit[k].scale = pool.scales[at_row * NB + (part >> 1)];
     }
   };
-  auto write = [&](int step) {
+  auto write = [&](int step, auto stage) {
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const int u = static_cast<int>(threadIdx.x) + kThreads * k;
@@ -242,7 +242,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_mx_shared_kernel(MxPrefil
       const bool seen = 32 * step + row < end;
       const uint2 c = seen ? unit[k].codes : make_uint2(0, 0);
       const float scale = mx_scale(seen ? unit[k].scale : 127);
-      uint8_t *to = ring[step & 1][of_v];
+      uint8_t *to = ring[decltype(stage)::value][of_v];
       const uint4 lo = make_uint4(pair_bits<0>(c.x, scale), pair_bits<1>(c.x, scale),
                                   pair_bits<2>(c.x, scale), pair_bits<3>(c.x, scale));
       const uint4 hi = make_uint4(pair_bits<0>(c.y, scale), pair_bits<1>(c.y, scale),
@@ -253,9 +253,9 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_mx_shared_kernel(MxPrefil
   };
 
   // Lane (g, i): scores of keys 16 h + 4 g + r, so V's operand is rows 4 g + r of both halves.
-  auto compute = [&](int step, auto whole_tile) {
+  auto compute = [&](int step, auto stage, auto whole_tile) {
     constexpr bool whole = decltype(whole_tile)::value;
-    const uint8_t *ks = ring[step & 1][0], *vs = ring[step & 1][1];
+    const uint8_t *ks = ring[decltype(stage)::value][0], *vs = ring[decltype(stage)::value][1];
     auto hidden = [&](int e) {
       return !whole && 32 * step + 16 * (e >> 2) + 4 * g + (e & 3) >= at.limit;
     };
@@ -307,25 +307,28 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_mx_shared_kernel(MxPrefil
   if constexpr (PAGED16) look_up(0);
   if (steps > 0) {
     load(0);
-    write(0);
+    write(0, std::integral_constant<int, 0>());
     load(min(1, steps - 1));
   }
   lds_barrier();
-  for (int step = 0; step < steps; ++step) {
+  auto turn = [&](int step, auto stage) {
     if (32 * step + 32 <= whole_end)
-      compute(step, std::true_type{});
+      compute(step, stage, std::true_type{});
     else if (32 * step < wave_end)
-      compute(step, std::false_type{});
+      compute(step, stage, std::false_type{});
     if (step + 1 < steps) {
-      write(step + 1);
+      write(step + 1, std::integral_constant<int, 1 - decltype(stage)::value>());
       const int next = min(step + 2, steps - 1);
       if constexpr (PAGED16)
         if (next >= looked_up + kLookUp) look_up(looked_up += kLookUp);
       load(next);
     }
     lds_barrier();
+  };
+  for (int step = 0; step < steps; step += 2) {
+    turn(step, std::integral_constant<int, 0>());
+    if (step + 1 < steps) turn(step + 1, std::integral_constant<int, 1>());
   }
-
   if (!r.live) return;
   const float sum = xgroup_sum(at.l);
   const float by = at.limit > 0 ? 1.f / sum : 0.f;  // (a row of no keys: zeros)
