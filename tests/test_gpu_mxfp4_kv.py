@@ -412,6 +412,66 @@ def test_attention_of_any_scale(device, sizes, chunks, scale) -> None:
         _check_attention(out[b:b + 1], query[b:b + 1], *pool.rows[b], scale)
 
 
+def test_refused_appends_and_gathers(device) -> None:
+    """By the operators themselves; nothing is written."""
+
+    def on(*shape, dtype=torch.float32):
+        return torch.zeros(shape, dtype=torch.uint8 if dtype.itemsize == 1 else dtype,
+                           device=device).view(dtype)
+
+    def pools(dh=64, dtype=CODES):
+        return on(1, 4, 2, 16, dh // 2, dtype=dtype), on(1, 4, 2, 16, dh // 2, dtype=dtype)
+
+    rows, slots = on(3, 2, 64) + 1, on(3, dtype=torch.int64)
+    kv = pools()
+    scales = {n: on(1, 4, 2, 16, 2, dtype=SCALES) for n in ("k_scales", "v_scales")}
+
+    def refused(kind, match, *args, **kw):
+        with pytest.raises(kind, match=match):
+            ops.kv_append(*args, **kw)
+
+    refused(ValueError, "need k_scales and v_scales", rows, rows, *kv, slots, 0)
+    refused(ValueError, "go together", rows, rows, *kv, slots, 0, k_scales=scales["k_scales"])
+    refused(TypeError, "float8_e8m0fnu", rows, rows, *kv, slots, 0, k_scales=scales["k_scales"],
+            v_scales=on(1, 4, 2, 16, 2))
+    refused(ValueError, "Dh / 32", rows, rows, *kv, slots, 0, k_scales=scales["k_scales"],
+            v_scales=on(1, 4, 2, 16, dtype=SCALES))
+    refused(ValueError, "head_dim of 32", on(3, 2, 160), on(3, 2, 160), *pools(160), slots, 0,
+            **scales)
+    refused(ValueError, "fp8 KV pools only", rows, rows, *kv, slots, 0, k_scale=2.0, **scales)
+    refused(ValueError, "must match the pool's", on(3, 2, 32), on(3, 2, 32), *kv, slots, 0, **scales)
+    refused(ValueError, "same dtype", rows, rows, kv[0], on(1, 4, 2, 16, 32, dtype=torch.uint8),
+            slots, 0, **scales)
+    refused(ValueError, "contiguous", rows, rows, *(p[:, ::2] for p in kv), slots, 0, **scales)
+    refused(ValueError, "storage dtype", rows, rows.half(), *kv, slots, 0, **scales)
+    refused(ValueError, "storage dtype", rows.double(), rows.double(), *kv, slots, 0, **scales)
+    refused(ValueError, "slot_mapping must have shape", rows, rows, *kv, slots[:2], 0, **scales)
+    refused(TypeError, "slot_mapping must be torch.int64", rows, rows, *kv, slots.int(), 0, **scales)
+    refused(ValueError, "requires HIP device", rows.cpu(), rows, *kv, slots, 0, **scales)
+    refused(ValueError, "requires HIP device", rows, rows, *kv, slots.cpu(), 0, **scales)
+    refused(IndexError, None, rows, rows, *kv, slots, 1, **scales)
+    tables, lens, cu = (on(*s, dtype=torch.int32) for s in ((2, 3), (2,), (3,)))
+    out = on(5, 2, 64), on(5, 2, 64)
+
+    def no_gather(kind, match, *args, **kw):
+        with pytest.raises(kind, match=match):
+            ops.paged_gather(*args, **kw)
+
+    no_gather(ValueError, "block_tables must have", *kv, tables[0], lens, cu, 0, 40, *out, **scales)
+    no_gather(TypeError, "seq_lens must be torch.int32", *kv, tables, lens.long(), cu, 0, 40, *out,
+              **scales)
+    no_gather(ValueError, "an entry per row", *kv, tables, lens[:1], cu, 0, 40, *out, **scales)
+    no_gather(ValueError, "outputs must have shape", *kv, tables, lens, cu, 0, 40, out[0][..., :32],
+              out[1][..., :32], **scales)
+    no_gather(ValueError, "share shape and strides", *kv, tables, lens, cu, 0, 40, out[0],
+              out[1][:4], **scales)
+    no_gather(ValueError, "outputs must match", *kv, tables, lens, cu, 0, 40, out[0], out[1].half(),
+              **scales)
+    no_gather(ValueError, None, *kv, tables, lens, cu, 0, 49, *out, **scales)  # (past the tables)
+    for t in (*kv, *scales.values()):
+        assert not t.view(torch.uint8).any()
+
+
 # ------------------------------------------------------ the operators together
 
 

@@ -371,13 +371,76 @@ void rope_kv_append_(const Tensor &query, const Tensor &key, const Tensor &value
                  layer_index, query, key_out, k_scale, v_scale, k_scales, v_scales);
 }
 
-void kv_append(const Tensor &key, const Tensor &value, const Tensor &key_cache,
+// The MXFP4 matrix operators and the cache's over MXFP4 pools check their arguments here (Python
+// does the same for traced calls): there the checks of a small product took 5 us of its 12.6,
+// those of an append and a gather 11 of 21.
+bool is_float(const Tensor &t) {
+  return t.scalar_type() == at::kFloat || t.scalar_type() == at::kHalf ||
+         t.scalar_type() == at::kBFloat16;
+}
+
+void one_device(const char *op, const Tensor &first, std::initializer_list<const Tensor *> others) {
+  TORCH_CHECK_VALUE(first.is_cuda(), op, " requires HIP device tensors");
+  for (const Tensor *t : others) {
+    if (t == nullptr) continue;
+    TORCH_CHECK_VALUE(t->is_cuda(), op, " requires HIP device tensors");
+    TORCH_CHECK_VALUE(t->device() == first.device(), op, ": tensors must use the same device");
+  }
+}
+
+const Tensor *maybe(const OptTensor &t) { return t ? &*t : nullptr; }
+
+void check_mxfp4_pools(const char *op, const Tensor &kc, const Tensor &vc,
+                       const OptTensor &k_scales, const OptTensor &v_scales) {
+  TORCH_CHECK_VALUE(kc.dim() == 5 && kc.sizes() == vc.sizes(),
+                    "KV pools must both have shape (L, NB, Hkv, BS, Dh)");
+  TORCH_CHECK_VALUE(kc.scalar_type() == vc.scalar_type(), "KV pools must use the same dtype");
+  TORCH_CHECK_VALUE(kc.is_contiguous() && vc.is_contiguous(), "KV pools must be contiguous");
+  const int64_t half = kc.size(4);
+  TORCH_CHECK_VALUE(half % 16 == 0 && half >= 16 && half <= 64,
+                    "MXFP4 KV pools need a head_dim of 32, 64, 96 or 128");
+  TORCH_CHECK_VALUE(k_scales || v_scales, op, ": MXFP4 KV pools need k_scales and v_scales");
+  TORCH_CHECK_VALUE(k_scales && v_scales, op, ": k_scales and v_scales go together");
+  for (const Tensor *t : {&*k_scales, &*v_scales}) {
+    const char *name = t == &*k_scales ? "k_scales" : "v_scales";
+    TORCH_CHECK_TYPE(t->scalar_type() == at::kFloat8_e8m0fnu, name,
+                     " of MXFP4 pools must be float8_e8m0fnu");
+    TORCH_CHECK_VALUE(t->dim() == 5 && t->sizes().slice(0, 4) == kc.sizes().slice(0, 4) &&
+                          t->size(4) == half / 16 && t->is_contiguous(),
+                      name, " must be a contiguous (L, NB, Hkv, BS, Dh / 32) tensor");
+  }
+}
+
+Tensor int_tensor(const Tensor &t, at::ScalarType type, const char *name) {
+  TORCH_CHECK_TYPE(t.scalar_type() == type, name, " must be torch.",
+                   type == at::kLong ? "int64" : "int32");
+  return t.contiguous();
+}
+
+void kv_append(const Tensor &key_rows, const Tensor &value_rows, const Tensor &key_cache,
                const Tensor &value_cache, const Tensor &slot_mapping, int64_t layer_index,
                double k_scale, double v_scale, const OptTensor &k_scales,
                const OptTensor &v_scales) {
+  const Tensor &kc = key_cache;
+  Tensor key = key_rows, value = value_rows, slots = slot_mapping;
+  if (mxfp4(kc)) {
+    const char *op = "kv_append";
+    one_device(op, key, {&value, &kc, &value_cache, &slots, maybe(k_scales), maybe(v_scales)});
+    check_mxfp4_pools(op, kc, value_cache, k_scales, v_scales);
+    TORCH_CHECK_VALUE(key.dim() == 3 && key.sizes() == value.sizes(),
+                      "key and value must have shape (N, Hkv, Dh)");
+    TORCH_CHECK_VALUE(key.size(1) == kc.size(2) && key.size(2) == 2 * kc.size(4),
+                      "key rows must match the pool's (Hkv, Dh)");
+    TORCH_CHECK_VALUE(is_float(key) && value.scalar_type() == key.scalar_type(),
+                      "keys and values must match the storage dtype");
+    TORCH_CHECK_VALUE(slots.dim() == 1 && slots.size(0) == key.size(0),
+                      "slot_mapping must have shape (N,)");
+    slots = int_tensor(slots, at::kLong, "slot_mapping");
+    if (key.stride(2) != 1) key = key.contiguous();
+    if (value.stride(2) != 1) value = value.contiguous();
+  }
   const c10::DeviceGuard guard(key.device());
   const Library &l = library();
-  const Tensor &kc = key_cache;
   auto call = [&](auto entry, auto scales, auto... factors) {
     return std::apply(
         [&](auto... rows) {
@@ -385,7 +448,7 @@ void kv_append(const Tensor &key, const Tensor &value, const Tensor &key_cache,
                        value.const_data_ptr(), value.stride(0), value.stride(1), key.size(0),
                        kc.mutable_data_ptr(), value_cache.mutable_data_ptr(), rows...,
                        i32(kc.size(0)), kc.size(1), i32(kc.size(2)), i32(kc.size(3)),
-                       head_dim(kc), i32(layer_index), as<int64_t>(slot_mapping), factors...,
+                       head_dim(kc), i32(layer_index), as<int64_t>(slots), factors...,
                        code(key), stream_of(key));
         },
         scales);
@@ -400,14 +463,36 @@ void kv_append(const Tensor &key, const Tensor &value, const Tensor &key_cache,
         "kv_append");
 }
 
-void paged_gather(const Tensor &key_cache, const Tensor &value_cache, const Tensor &block_tables,
-                  const Tensor &seq_lens, const Tensor &cu_seqlens, int64_t layer_index,
+void paged_gather(const Tensor &key_cache, const Tensor &value_cache, const Tensor &tables,
+                  const Tensor &lens, const Tensor &cu, int64_t layer_index,
                   int64_t max_seq_len, const Tensor &key_out, const Tensor &value_out,
                   double k_scale, double v_scale, const OptTensor &k_scales,
                   const OptTensor &v_scales) {
+  const Tensor &kc = key_cache;
+  Tensor block_tables = tables, seq_lens = lens, cu_seqlens = cu;
+  if (mxfp4(kc)) {
+    const char *op = "paged_gather";
+    one_device(op, kc, {&value_cache, &tables, &lens, &cu, &key_out, &value_out, maybe(k_scales),
+                        maybe(v_scales)});
+    check_mxfp4_pools(op, kc, value_cache, k_scales, v_scales);
+    TORCH_CHECK_VALUE(tables.dim() == 2, "block_tables must have shape (B, max_blocks)");
+    block_tables = int_tensor(tables, at::kInt, "block_tables");
+    seq_lens = int_tensor(lens, at::kInt, "seq_lens");
+    cu_seqlens = int_tensor(cu, at::kInt, "cu_seqlens");
+    TORCH_CHECK_VALUE(lens.numel() >= tables.size(0) && cu.numel() >= tables.size(0),
+                      "seq_lens and cu_seqlens must have an entry per row of block_tables");
+    TORCH_CHECK_VALUE(key_out.dim() == 3 && key_out.size(1) == kc.size(2) &&
+                          key_out.size(2) == 2 * kc.size(4),
+                      "outputs must have shape (S, Hkv, Dh)");
+    TORCH_CHECK_VALUE(value_out.sizes() == key_out.sizes() &&
+                          value_out.strides() == key_out.strides(),
+                      "key_out and value_out must share shape and strides");
+    TORCH_CHECK_VALUE(key_out.stride(2) == 1, "outputs must be contiguous in head_dim");
+    TORCH_CHECK_VALUE(is_float(key_out) && value_out.scalar_type() == key_out.scalar_type(),
+                      "outputs must match the storage dtype");
+  }
   const c10::DeviceGuard guard(key_cache.device());
   const Library &l = library();
-  const Tensor &kc = key_cache;
   auto call = [&](auto entry, auto scales, auto... factors) {
     return std::apply(
         [&](auto... rows) {
@@ -453,22 +538,6 @@ void silu_mul(const Tensor &gate_up, const Tensor &out) {
                                gate_up.size(1) / 2, out.mutable_data_ptr(), out.stride(0),
                                code(gate_up), stream_of(gate_up)),
         "silu_mul");
-}
-
-// The MXFP4 matrix operators check their arguments here (torch_ops.py does the same for
-// traced calls): in Python the checks of a small product took 5 us of its 12.6.
-bool is_float(const Tensor &t) {
-  return t.scalar_type() == at::kFloat || t.scalar_type() == at::kHalf ||
-         t.scalar_type() == at::kBFloat16;
-}
-
-void one_device(const char *op, const Tensor &first, std::initializer_list<const Tensor *> others) {
-  TORCH_CHECK_VALUE(first.is_cuda(), op, " requires HIP device tensors");
-  for (const Tensor *t : others) {
-    if (t == nullptr) continue;
-    TORCH_CHECK_VALUE(t->is_cuda(), op, " requires HIP device tensors");
-    TORCH_CHECK_VALUE(t->device() == first.device(), op, ": tensors must use the same device");
-  }
 }
 
 bool same_lead(const Tensor &a, const Tensor &b) {
@@ -517,8 +586,6 @@ void check_space(const char *op, const OptTensor &workspace) {
                                    workspace->is_contiguous()),
                     op, ": workspace must be a contiguous uint8 tensor");
 }
-
-const Tensor *maybe(const OptTensor &t) { return t ? &*t : nullptr; }
 
 // Rows and row stride of a matrix whose last dimension is `width` long and contiguous (of
 // other than two dimensions: contiguous).

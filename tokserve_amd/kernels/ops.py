@@ -144,6 +144,14 @@ def _row_scales(
     return k_scales, v_scales
 
 
+def _natively_checked(pool: torch.Tensor, k_scale: float, v_scale: float) -> bool:
+    """Whether the cache's operators check a call themselves: over MXFP4 pools, on the device.
+    (Traced calls are checked in Python.)"""
+
+    return (pool.dtype == MXFP4_DTYPE and type(pool) is torch.Tensor and k_scale == 1.0
+            and v_scale == 1.0 and pool.is_cuda and not torch.compiler.is_compiling())
+
+
 def _last_dim_contiguous(tensor: torch.Tensor, name: str) -> torch.Tensor:
     return tensor if tensor.stride(-1) == 1 else tensor.contiguous()
 
@@ -181,6 +189,10 @@ def kv_append(
     that dtype, copied bit for bit.
     """
 
+    if _natively_checked(key_cache, k_scale, v_scale) and key.is_cuda:
+        _ops.kv_append(key, value, key_cache, value_cache, slot_mapping, layer_index, 1.0, 1.0,
+                       k_scales, v_scales)
+        return
     require_hip("kv_append", key, value, key_cache, value_cache, slot_mapping)
     num_layers, num_blocks, num_kv_heads, block_size, head_dim = _pool_shape(
         key_cache, value_cache
@@ -227,6 +239,10 @@ def paged_gather(
     k_scales / v_scales) into the outputs' float dtype.
     """
 
+    if _natively_checked(key_cache, k_scale, v_scale):
+        _ops.paged_gather(key_cache, value_cache, block_tables, seq_lens, cu_seqlens, layer_index,
+                          max_seq_len, key_out, value_out, 1.0, 1.0, k_scales, v_scales)
+        return
     require_hip(
         "paged_gather", key_cache, value_cache, block_tables, seq_lens, cu_seqlens,
         key_out, value_out,
