@@ -455,7 +455,8 @@ int32_t tks_mxfp4_matmul(const void *a_codes, const void *a_scales, const void *
 
 /* A projection with MXFP4 weights: rows of `dtype` are quantized as
  * tks_mxfp4_quantize does and multiplied as tks_mxfp4_matmul does; the results are the
- * two calls' up to the order of their fp32 sums. Workspace as for the product, from its own size query. */
+ * two calls' up to the order of their fp32 sums. `out` must not overlap `input`.
+ * Workspace as for the product, from its own size query. */
 int64_t tks_mxfp4_linear_workspace_bytes(int64_t num_rows, int64_t num_cols, int64_t depth);
 
 int32_t tks_mxfp4_linear(const void *input, int64_t input_row_stride, const void *weight_codes,
@@ -499,8 +500,9 @@ int32_t tks_rope_kv_append_mxfp4(
     int32_t layer_index, const int64_t *slot_mapping, int32_t dtype, tks_stream_t stream);
 
 /* Decode attention: the function of tks_paged_attention_decode on the decoded pools
- * (exact values, products and sums in fp32). At most 16 query heads to a KV head.
- * Workspace of tks_paged_attention_decode_workspace_bytes. */
+ * (exact values; scores exact products summed in fp32; probabilities of 8, 16 or 24
+ * bits for bf16, fp16 and fp32 queries, summed in fp32). At most 16 query heads to a KV
+ * head. A NaN block makes its outputs NaN where a query sees it. Workspace of tks_paged_attention_decode_workspace_bytes. */
 int32_t tks_paged_attention_decode_mxfp4(
     const void *query, int64_t q_seq_stride, int64_t q_head_stride, const void *key_cache,
     const void *value_cache, const void *k_scales, const void *v_scales, int32_t num_layers,
@@ -525,7 +527,7 @@ int32_t tks_rope_append_paged_decode_mxfp4(
     int32_t pages_per_split, void *out, int64_t out_seq_stride, int64_t out_head_stride,
     void *workspace, int64_t workspace_bytes, int32_t dtype, tks_stream_t stream);
 
-/* Chunked-prefill attention. Batches of many rows (a query token times a head of the group)
+/* Chunked-prefill attention, as the decode. Batches of many rows (a query token times a head of the group)
  * per sequence and KV head need a workspace, 0 bytes otherwise: the pages they read are
  * decoded into it (a dense pool in `dtype` of ceil(max_seq_len / block_size) pages to a
  * sequence, values rounded once to it; 16-byte aligned). */

@@ -285,3 +285,25 @@ def test_nan_blocks_of_a_long_depth(device, m, k) -> None:
     bad[5] = True
     bad[:, 90] = True
     assert torch.equal(out.isnan(), bad)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 500, 2048), (40, 96, 544), (70, 130, 2080), (300, 200, 1024)])
+def test_projections_on_two_streams(device, m, n, k) -> None:
+    """Calls at once, each with scratch memory of its own, and with a workspace for each."""
+
+    w = ops.mxfp4_quantize(_rows(n, k, torch.float32, 1, spread=3).to(device))
+    inputs = [_rows(m, k, torch.bfloat16, s, spread=3).to(device) for s in (2, 3)]
+    want = [ops.mxfp4_linear(x, *w) for x in inputs]
+    size = ops.mxfp4_linear_workspace_bytes(m, n, k)
+    spaces = [torch.empty(size + 16, dtype=torch.uint8, device=device) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    results = []
+    for turn in range(12):
+        i = turn % 2
+        with torch.cuda.stream(streams[i]):
+            results.append((i, ops.mxfp4_linear(inputs[i], *w,
+                                                workspace=spaces[i] if turn % 4 < 2 else None)))
+    torch.cuda.synchronize()
+    for i, got in results:
+        assert torch.equal(got, want[i])

@@ -475,6 +475,58 @@ def test_refused_appends_and_gathers(device) -> None:
 # ------------------------------------------------------ the operators together
 
 
+@pytest.mark.parametrize("sizes,chunks", [FORMS[0], FORMS[3], FORMS[10]])
+def test_attention_from_graphs_and_on_two_streams(device, sizes, chunks) -> None:
+    """A prefill of each form and a split decode: captured and replayed among eager calls, and
+    two at once on two streams, each with scratch memory of its own."""
+
+    hq, hkv, dh, block_size = sizes
+    lengths = [t + p for t, p in chunks]
+    new = [t for t, _ in chunks]
+    pools = [Pool(lengths, hkv, dh, block_size, device, seed=s) for s in (1, 2)]
+    cu = torch.tensor([0, *torch.tensor(new).cumsum(0).tolist()], dtype=torch.int32, device=device)
+    g = torch.Generator().manual_seed(3)
+    queries = [torch.randn(sum(new), hq, dh, generator=g).bfloat16().to(device) for _ in range(2)]
+
+    def both(pool, query):
+        out = ops.paged_attention_prefill(
+            query, pool.key, pool.value, pool.block_tables, pool.lens, cu, layer_index=0,
+            max_query_len=max(new), max_seq_len=max(lengths), **pool.scales)
+        last = ops.paged_attention_decode(
+            query[:len(new)], pool.key, pool.value, pool.block_tables, pool.lens, layer_index=0,
+            max_seq_len=max(lengths), pages_per_split=2, **pool.scales)
+        return out, last
+
+    want = [[both(pool, query) for query in queries] for pool in pools]
+    torch.cuda.synchronize()
+    graphs = []
+    for pool in pools:
+        static = queries[0].clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = both(pool, static)
+        graphs.append((graph, static, out))
+    for turn in range(4):
+        for i, (graph, static, out) in enumerate(graphs):
+            static.copy_(queries[turn % 2])
+            graph.replay()
+            eager = both(pools[1 - i], queries[turn % 2])
+            torch.cuda.synchronize()
+            for a, b in zip((*out, *eager), (*want[i][turn % 2], *want[1 - i][turn % 2])):
+                assert torch.equal(a, b)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    results = []
+    for turn in range(6):
+        i = turn % 2
+        streams[i].wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(streams[i]):
+            results.append((i, both(pools[i], queries[i])))
+    torch.cuda.synchronize()
+    for i, got in results:
+        for a, b in zip(got, want[i][i]):
+            assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_a_cache_through_its_life(device, dtype) -> None:
     """Prefill in two chunks, then decode steps, through the storage: every step attends to

@@ -10,7 +10,6 @@
 #include "rope_common.hpp"
 
 #include <algorithm>
-
 #include <type_traits>
 
 namespace tks {

@@ -179,7 +179,8 @@ def kv_append(
     k_scales: torch.Tensor | None = None,
     v_scales: torch.Tensor | None = None,
 ) -> None:
-    """Scatter K/V rows (N, Hkv, Dh) into the pools at slot_mapping (int64, N).
+    """Scatter K/V rows (N, Hkv, Dh) into the pools at slot_mapping (int64, N; distinct, or
+    negative for rows to leave out).
 
     fp8 pools quantize the rows with the pool scales (k_scale, v_scale), or, given
     k_scales / v_scales (float32 (L, NB, Hkv, BS)), each row with a scale of its
@@ -585,7 +586,8 @@ def mxfp4_linear(
     """A projection with MXFP4 weights (N, K): inputs (..., K) -> (..., N) in their dtype.
 
     The rows are quantized as mxfp4_quantize does and multiplied as mxfp4_matmul does;
-    the results are the two calls' up to the order of their fp32 sums. `workspace` as there, of mxfp4_linear_workspace_bytes.
+    the results are the two calls' up to the order of their fp32 sums. `out` must not overlap
+    `inputs`. `workspace` as there, of mxfp4_linear_workspace_bytes.
     """
 
     device = require_hip("mxfp4_linear", inputs)
