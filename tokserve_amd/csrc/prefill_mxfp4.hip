@@ -176,14 +176,12 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_mx_shared_kernel(MxPrefil
   const int G = a.group;
   const Work w = work_of(a, kRows);
   if (w.row0 >= w.rows) return;
-  const int64_t row0 = w.row0 + 16 * wave;
-  // Keys that the workgroup's rows, the wave's rows and every one of the wave's rows see.
+  // Keys that some and that every row of the workgroup sees.
   const int end = max(seen_by(w, min(w.row0 + kRows, w.rows) - 1, G), 0);
-  const int wave_end = row0 < w.rows ? seen_by(w, min(row0 + 16, w.rows) - 1, G) : 0;
-  const int whole_end = row0 < w.rows ? seen_by(w, row0, G) : 0;
+  const int whole_end = max(seen_by(w, w.row0, G), 0);
 
   Rows<T, NB, PAGED16> r;
-  r.start(a, w, row0, g, i);
+  r.start(a, w, w.row0 + 16 * wave, g, i);
   auto &at = r.at;
 
   // A thread's units of a tile: 16 values of a row each. K's come first, then V's (a wave's are
@@ -205,51 +203,65 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_mx_shared_kernel(MxPrefil
               ((key - page * BS) >> 4);
     }
   };
-  auto load = [&](int step) {
-    int64_t page[2] = {0, 0};
-    if constexpr (PAGED16) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        page[h] = layer_row + 16 * static_cast<int64_t>(__builtin_amdgcn_readlane(
-                                       pages, 2 * (step & (kLookUp - 1)) + h));
-    }
+  auto page_row = [&](int step, int h) {
+    return layer_row + 16 * static_cast<int64_t>(__builtin_amdgcn_readlane(
+                                pages, 2 * (step & (kLookUp - 1)) + h));
+  };
+  auto each_unit = [&](auto f) {
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const int u = static_cast<int>(threadIdx.x) + kThreads * k;
       if (kUnits % kThreads != 0 && u >= kUnits) continue;
       const bool of_v = 64 * wave + kThreads * k >= 64 * NB;
-      const MxPool &pool = of_v ? a.vc : a.kc;
-      const int v = of_v ? u - 64 * NB : u, row = v / (2 * NB), part = v - row * (2 * NB);
-      int64_t at_row;
-      if constexpr (PAGED16) {
-        at_row = (row < 16 ? page[0] : page[1]) + (row & 15);
-      } else {
-        const int key = min(32 * step + row, end - 1), pg = key / BS;
-        at_row = a.kc.row(block_of(w.bt, pg, a.kc.num_blocks), w.kvh, key - pg * BS);
-      }
-      unit[k].codes = *reinterpret_cast<const uint2 *>(pool.codes + at_row * (16 * NB) + 8 * part);
-      unit[k].scale = pool.scales[at_row * NB + (part >> 1)];
+      const int v = of_v ? u - 64 * NB : u, row = v / (2 * NB);
+      f(unit[k], of_v, row, v - row * (2 * NB));
     }
   };
+  auto load = [&](int step) {
+    each_unit([&](Unit &x, bool of_v, int row, int part) {
+      const MxPool &pool = of_v ? a.vc : a.kc;
+      if constexpr (PAGED16 && NB % 2 == 0) {
+        // (A wave's rows are all of one page: its address in scalar registers.)
+        const int64_t from = page_row(step, __builtin_amdgcn_readfirstlane(row >> 4));
+        const uint32_t in = row & 15;
+        x.codes = *reinterpret_cast<const uint2 *>(pool.codes + from * (16 * NB) +
+                                                   (in * (16 * NB) + 8 * part));
+        x.scale = (pool.scales + from * NB)[in * NB + (part >> 1)];
+      } else {
+        int64_t from;
+        if constexpr (PAGED16) {
+          const int64_t first = page_row(step, 0), second = page_row(step, 1);
+          from = (row < 16 ? first : second) + (row & 15);
+        } else {
+          const int key = min(32 * step + row, end - 1), pg = key / BS;
+          from = a.kc.row(block_of(w.bt, pg, a.kc.num_blocks), w.kvh, key - pg * BS);
+        }
+        x.codes = *reinterpret_cast<const uint2 *>(pool.codes + from * (16 * NB) + 8 * part);
+        x.scale = pool.scales[from * NB + (part >> 1)];
+      }
+    });
+  };
   auto write = [&](int step, auto stage) {
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int u = static_cast<int>(threadIdx.x) + kThreads * k;
-      if (kUnits % kThreads != 0 && u >= kUnits) continue;
-      const bool of_v = 64 * wave + kThreads * k >= 64 * NB;
-      const int v = of_v ? u - 64 * NB : u, row = v / (2 * NB), part = v - row * (2 * NB);
-      // (Keys that no row sees are zeros: what the pool has there may be NaN.)
-      const bool seen = 32 * step + row < end;
-      const uint2 c = seen ? unit[k].codes : make_uint2(0, 0);
-      const float scale = mx_scale(seen ? unit[k].scale : 127);
+    each_unit([&](Unit &x, bool of_v, int row, int part) {
+      if (32 * step + 32 > end && 32 * step + row >= end) {
+        // (Keys that no row sees are zeros: what the pool has there may be NaN.)
+        x.codes = make_uint2(0, 0);
+        x.scale = 127;
+      }
+      // Half of the lanes write their second chunk first, so that eight lanes' are of eight
+      // different bank groups.
+      const bool second = NB == 2 ? !of_v && (row & 1) : NB == 4 && part >= 4;
+      const uint32_t c0 = second ? x.codes.y : x.codes.x, c1 = second ? x.codes.x : x.codes.y;
+      const int chunk = 2 * part + second;
+      const float scale = mx_scale(x.scale);
       uint8_t *to = ring[decltype(stage)::value][of_v];
-      const uint4 lo = make_uint4(pair_bits<0>(c.x, scale), pair_bits<1>(c.x, scale),
-                                  pair_bits<2>(c.x, scale), pair_bits<3>(c.x, scale));
-      const uint4 hi = make_uint4(pair_bits<0>(c.y, scale), pair_bits<1>(c.y, scale),
-                                  pair_bits<2>(c.y, scale), pair_bits<3>(c.y, scale));
-      st16(to + (of_v ? Keys::v_at(row, 2 * part) : Keys::k_at(row, 2 * part)), lo);
-      st16(to + (of_v ? Keys::v_at(row, 2 * part + 1) : Keys::k_at(row, 2 * part + 1)), hi);
-    }
+      st16(to + (of_v ? Keys::v_at(row, chunk) : Keys::k_at(row, chunk)),
+           make_uint4(pair_bits<0>(c0, scale), pair_bits<1>(c0, scale), pair_bits<2>(c0, scale),
+                      pair_bits<3>(c0, scale)));
+      st16(to + (of_v ? Keys::v_at(row, chunk ^ 1) : Keys::k_at(row, chunk ^ 1)),
+           make_uint4(pair_bits<0>(c1, scale), pair_bits<1>(c1, scale), pair_bits<2>(c1, scale),
+                      pair_bits<3>(c1, scale)));
+    });
   };
 
   // Lane (g, i): scores of keys 16 h + 4 g + r, so V's operand is rows 4 g + r of both halves.
@@ -311,11 +323,8 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_mx_shared_kernel(MxPrefil
     load(min(1, steps - 1));
   }
   lds_barrier();
-  auto turn = [&](int step, auto stage) {
-    if (32 * step + 32 <= whole_end)
-      compute(step, stage, std::true_type{});
-    else if (32 * step < wave_end)
-      compute(step, stage, std::false_type{});
+  auto turn = [&](int step, auto stage, auto whole_tile) {
+    compute(step, stage, whole_tile);
     if (step + 1 < steps) {
       write(step + 1, std::integral_constant<int, 1 - decltype(stage)::value>());
       const int next = min(step + 2, steps - 1);
@@ -325,9 +334,18 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_mx_shared_kernel(MxPrefil
     }
     lds_barrier();
   };
-  for (int step = 0; step < steps; step += 2) {
-    turn(step, std::integral_constant<int, 0>());
-    if (step + 1 < steps) turn(step + 1, std::integral_constant<int, 1>());
+  typedef std::integral_constant<int, 0> Even;
+  typedef std::integral_constant<int, 1> Odd;
+  // (Two loops, not a choice in one: it would have the sums copied from path to path.)
+  const int whole = whole_end / 64 * 2;  // tiles that every row sees, in pairs
+  int step = 0;
+  for (; step < whole; step += 2) {
+    turn(step, Even(), std::true_type{});
+    turn(step + 1, Odd(), std::true_type{});
+  }
+  for (; step < steps; step += 2) {
+    turn(step, Even(), std::false_type{});
+    if (step + 1 < steps) turn(step + 1, Odd(), std::false_type{});
   }
   if (!r.live) return;
   const float sum = xgroup_sum(at.l);
