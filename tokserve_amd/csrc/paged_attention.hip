@@ -1350,10 +1350,10 @@ namespace {
 // for the kernel of the 16-bit pools: two launches more, and nine tenths to two thirds of the
 // time where a (sequence, KV head) has enough rows, and rows times keys, to pay for them. us so
 // and straight from the pools (prefill_mxfp4.hip), 32 heads: bf16, 8 KV heads of Dh 128, 16 x 512
-// tokens after up to 2,048 keys 278 and 335 (2,048 rows), 16 x 256 after 4,096 240 and 269 (1,024),
+// tokens after up to 2,048 keys 282 and 324 (2,048 rows), 16 x 256 after 4,096 240 and 269 (1,024),
 // 4 x 256 after none 23 and 22, 16 x 128 after 4,096 160 and 147 (512), 64 x 64 381 and 259 (256);
 // fp16 16 x 256 243 and 377, 64 x 64 384 and 364; bf16, 4 KV heads of Dh 64, 16 x 512 after up to
-// 2,048 162 and 180 (4,096 rows, 10M), 8 x 512 after none 49 and 40 (2M), 4 x 100-300 after up to 300
+// 2,048 160 and 182 (4,096 rows, 10M), 8 x 512 after none 49 and 37 (2M), 4 x 100-300 after up to 300
 // 22 and 19 (1M). Not for more than kMaxDecoded bytes of it.
 constexpr int64_t kDecodedRows = 1024;
 constexpr int64_t kDecodedWork = int64_t{1} << 19, kDecodedWork64 = int64_t{1} << 22;

@@ -7,8 +7,9 @@
 //  * shared: the four waves of a workgroup take different rows and walk the same keys. A tile
 //    of 32 keys is decoded once, to bf16 in LDS ([key][dim], double-buffered, one barrier a
 //    tile), while the next one's codes are on their way to registers; V's operand comes out of
-//    it transposed (ds_read_b64_tr_b16). What bounds it is the vector ALU (an exponential per
-//    score, the decoding) and the waits around the barrier.
+//    it transposed (ds_read_b64_tr_b16). What bounds it is a tile's chain (scores, softmax,
+//    values, barrier), which three waves per SIMD do not cover: bf16, 16 x 512 tokens, Dh 128,
+//    324 us, the matrix pipe busy a quarter of it. Tiles of 64 keys are level.
 //  * apart: the four waves take the same rows, the tiles of keys dealt round, each decoding
 //    its own in registers; their sums meet in LDS. Where there are few rows the longest chain
 //    of tiles sets the time, and this quarters it.
@@ -16,7 +17,7 @@
 // us of each (apart, shared), kv heads 8 of Dh 128 under 32 heads, 4,096 earlier keys: bf16 4 x
 // 128 tokens 44, 109; 16 x 64 85, 115; 16 x 128 163, 147; 512 earlier keys: 4 x 128 22, 26; 16 x
 // 64 35, 27; fp32 5 x 1-333 tokens, Dh 64, to 1,024 earlier: 23, 32 (over decoded fp32 pages, as
-// before these: 61); fp32 16 x 512, Dh 128, to 2,048 earlier: 642, 594 (1,590); bf16 4 x 200-400,
+// before these: 61); fp32 16 x 512, Dh 128, to 2,048 earlier: 642, 573 (1,590); bf16 4 x 200-400,
 // Dh 96, to 1,024 earlier: 76, 45 (3,910: nothing but a plain kernel takes such pages).
 #include "mxfp4_attention.hpp"
 
