@@ -470,7 +470,8 @@ int32_t tks_mxfp4_linear(const void *input, int64_t input_row_stride, const void
  * `head_dim` is Dh. Each entry takes the arguments of its *_fp8_rows counterpart
  * with the scale bytes in place of the fp32 scales; `dtype` is the type of the other
  * tensors (new rows, gathered rows, query, output). Rows no sequence has written
- * are never read into an output. */
+ * are never read into an output. The attention's block sizes are multiples of 16, or a
+ * layer has fewer than 2^31 rows (num_blocks * num_kv_heads * block_size). */
 int32_t tks_kv_append_mxfp4(const void *key, int64_t key_token_stride, int64_t key_head_stride,
                             const void *value, int64_t value_token_stride,
                             int64_t value_head_stride, int64_t num_tokens, void *key_cache,

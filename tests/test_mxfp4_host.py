@@ -176,6 +176,10 @@ def test_c_entries_check_before_any_launch() -> None:
                         64, 64, None, 0, 0, None]
     assert decode(*args(keys=65)) == value and decode(*args(heads=17)) == value
     assert decode(*args(pages=1)) == space
+    # A layer of 2^31 rows or more: blocks of 16 tokens only.
+    many = args(width=64)
+    many[8], many[10] = 1 << 31, 1
+    assert decode(*many) == value
     prefill = library.tks_paged_attention_prefill_mxfp4_workspace_bytes
     assert prefill(2, 4, 4, 1, 64, 16, 40, 0) == 0  # (fp32: straight from the pools)
     assert prefill(2, 511, 4, 1, 128, 16, 512, 2) == 0 == prefill(2, 512, 4, 1, 128, 16, 511, 2)

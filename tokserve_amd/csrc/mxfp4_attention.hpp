@@ -298,11 +298,16 @@ struct MxAttention {
                                       int stride, int lane) {
     const int g = lane >> 4, i = lane & 15;
     const int BS = kc.block_size;
-    // Pool row of a key (clamped to the last one: its loads are masked).
-    auto row_of = [&](int key) -> int64_t {
-      key = min(key, end - 1);
+    // Without PAGED16: rows (of this layer) of the keys of two of the wave's tiles, 2 pair and
+    // 2 pair + 1, a lane each; those of the next two are looked up meanwhile. (Past the end the
+    // last key's, masked.)
+    int rows = 0, next_rows = 0, pair = 0;
+    auto rows_of = [&](int of) {
+      const int tile = 2 * of + (lane >> 5);
+      const int key = min(begin + 32 * (first + stride * tile) + (lane & 31), end - 1);
       const int page = key / BS;
-      return kc.row(block_of(bt, page, kc.num_blocks), kvh, key - page * BS);
+      return static_cast<int>((block_of(bt, page, kc.num_blocks) * kc.num_kv_heads + kvh) * BS) +
+             key - page * BS;
     };
     // With PAGED16 a half tile is a page of 16 rows, id = pool row / 16 (of this layer): lane
     // 2 n + h holds that of half h of the wave's tile `from` + n, so that a table entry is read
@@ -334,11 +339,14 @@ struct MxAttention {
 #pragma unroll
           for (int r = 0; r < 4; ++r) load_v<NB>(vp, vs, 4 * r + g, i, t.v[h][r], t.vs[h][r]);
         } else {
-          const int64_t k_at = row_of(base_of(n) + 16 * h + k_row);
+          auto row_of = [&](int key) {  // of the tile
+            return layer_row + __builtin_amdgcn_ds_bpermute(4 * (32 * (n & 1) + key), rows);
+          };
+          const int64_t k_at = row_of(16 * h + k_row);
           load_k<NB>(kc.codes + k_at * (16 * NB), kc.scales + k_at * NB, 0, g, t.k[h], t.ks[h]);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int64_t at = row_of(base_of(n) + 16 * h + 4 * r + g);
+            const int64_t at = row_of(16 * h + 4 * r + g);
             load_v<NB>(vc.codes + at * (16 * NB), vc.scales + at * NB, 0, i, t.v[h][r],
                        t.vs[h][r]);
           }
@@ -357,11 +365,20 @@ struct MxAttention {
     // have to be waited for before the next one is worked on.)
     auto fetch = [&](int n, Tile<NB> &t) {
       n = min(n, mine - 1);
-      if constexpr (PAGED16)
+      if constexpr (PAGED16) {
         if (n >= looked_up + kLookUp) look_up(looked_up += kLookUp);
+      } else if (n >> 1 > pair) {
+        rows = next_rows;
+        next_rows = rows_of(++pair + 1);
+      }
       load(n, t);
     };
-    if constexpr (PAGED16) look_up(0);
+    if constexpr (PAGED16) {
+      look_up(0);
+    } else {
+      rows = rows_of(0);
+      next_rows = rows_of(1);
+    }
     load(0, even);
     int n = 0;
     for (; n + 1 < whole; n += 2) {

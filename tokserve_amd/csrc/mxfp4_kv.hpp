@@ -31,6 +31,11 @@ inline bool mx_pool_ok(int32_t num_layers, int64_t num_blocks, int32_t num_kv_he
   return num_layers > 0 && num_blocks > 0 && num_kv_heads > 0 && block_size > 0 &&
          head_dim > 0 && head_dim <= kMxMaxDh && head_dim % kMxBlock == 0;
 }
+// Attention over blocks that are no multiple of 16 numbers a layer's rows in 32 bits.
+inline bool mx_rows_ok(int64_t num_blocks, int32_t num_kv_heads, int32_t block_size) {
+  return block_size % 16 == 0 ||
+         num_blocks <= INT32_MAX / (static_cast<int64_t>(num_kv_heads) * block_size);
+}
 
 // Codes are read and written four bytes at a time at least, sixteen in the decode.
 inline bool mx_pools_given(const void *kc, const void *vc, const void *ks, const void *vs) {

@@ -1191,17 +1191,20 @@ namespace {
 // microsecond, whatever it waits for, so the merge (a launch, 3 us) pays later than over the
 // other pools; never more splits than choose_pages_per_split has, whose workspace query serves
 // both. us of bf16 queries at 32 / 8 heads, Dh 128 and 32 / 4, Dh 64 (blocks of 16):
-//  * A bound below 2,048 keys: unsplit. One sequence of 512 keys 6.1 and 5.6 (two splits 8.5
+//  * A bound below 1,280 keys: unsplit. One sequence of 512 keys 6.1 and 5.6 (two splits 8.5
 //    and 8.1), 16 of up to 1,152 8.4 and 7.3 (11.1 and 8.8).
-//  * Fewer than kFillItems pairs: 512 keys or what fills the CUs, up to 768 or an eighth of
-//    the bound. One sequence of 131,072 keys 31.6 (4,096-key splits; 54.8 at 768); one of up to 8,192
-//    10.3 and 9.7 at 512 keys, 11.9 and 11.2 at 256; 16 28.0 - 30 at any from 512 up.
-//  * Fewer than kSplitBelowItems: four keys per pair, or an eighth of the bound. Up to 8,192
-//    keys, log-uniform and from 4,096 up uniform: 256 pairs 23.3 and 44.5 at 1,024 keys, 25.4 and
-//    47.8 at 512, 32.5 and 47.2 at 2,048; 768 of Dh 64 42.5 and 86.1 at 4,096, 46.7 and 115.7 at 512.
+//  * Fewer than kFillItems pairs: a sixteenth of the bound, 256 to 512 keys, or what fills the
+//    CUs, up to 768 or an eighth of the bound. One sequence of 1,599 keys 8.3 (9.7 unsplit; fp32
+//    8.9 and 12.5), of 4,096 9.3 (10.1 at 512 keys), of up to 8,192 10.3 at 512 (11.9 at 256), of
+//    131,072 31.6 at 4,096 (54.8 at 768); 16 of up to 8,192 28 - 30 at any from 512 up.
+//  * Fewer than kSplitBelowItems, a bound of 1,280 or more: four keys per pair, or an eighth of the
+//    bound. Up to 8,192 keys, log-uniform and from 4,096 up uniform: 256 pairs 23.3 and 44.5 at
+//    1,024 keys, 25.4 and 47.8 at 512, 32.5 and 47.2 at 2,048; 768 of Dh 64 42.5 and 86.1 at 4,096,
+//    46.7 and 115.7 at 512.
 //  * Otherwise unsplit: 1,024 pairs 57.0 and 154, 62.0 and 188 at 1,024 keys.
-constexpr int64_t kMxSplitFrom = 2048;
-constexpr int64_t kMxMinSplit = 512, kMxFillSplit = 768, kMxSplitsOfBound = 8, kMxKeysPerItem = 4;
+constexpr int64_t kMxSplitFrom = 1280;
+constexpr int64_t kMxLeastSplit = 256, kMxMinSplit = 512, kMxMinOfBound = 16;
+constexpr int64_t kMxFillSplit = 768, kMxSplitsOfBound = 8, kMxKeysPerItem = 4;
 int32_t choose_pages_mxfp4(int32_t num_seqs, int32_t num_kv_heads, int32_t block_size,
                            int32_t max_seq_len, int32_t requested) {
   const int32_t pps = choose_pages_per_split(num_seqs, num_kv_heads, block_size, max_seq_len,
@@ -1213,7 +1216,9 @@ int32_t choose_pages_mxfp4(int32_t num_seqs, int32_t num_kv_heads, int32_t block
   int64_t keys = bound;
   if (bound >= kMxSplitFrom && items < kFillItems) {
     const int64_t fill = ceil_div(max_pages, ceil_div(kFillItems, items)) * block_size;
-    keys = std::min(std::max(kMxMinSplit, fill), std::max(kMxFillSplit, bound / kMxSplitsOfBound));
+    const int64_t least =
+        std::min(kMxMinSplit, std::max(kMxLeastSplit, bound / kMxMinOfBound));
+    keys = std::min(std::max(least, fill), std::max(kMxFillSplit, bound / kMxSplitsOfBound));
   } else if (bound >= kMxSplitFrom && items < kSplitBelowItems) {
     keys = std::max(kMxKeysPerItem * items, bound / kMxSplitsOfBound);
   }
@@ -1233,7 +1238,8 @@ int32_t decode_mxfp4_impl(const void *query, int64_t q_seq_stride, int64_t q_hea
   if (!valid_dtype(dtype)) return TKS_ERR_TYPE;
   if (!mx_pool_ok(num_layers, num_blocks, num_kv_heads, block_size, head_dim) || num_seqs < 0 ||
       num_q_heads <= 0 || num_q_heads % num_kv_heads != 0 || max_seq_len < 0 ||
-      pages_per_split < 0 || num_q_heads / num_kv_heads > kGenMaxG)
+      pages_per_split < 0 || num_q_heads / num_kv_heads > kGenMaxG ||
+      !mx_rows_ok(num_blocks, num_kv_heads, block_size))
     return TKS_ERR_VALUE;
   if (layer_index < 0 || layer_index >= num_layers) return TKS_ERR_INDEX;
   if (num_seqs == 0) return TKS_OK;
@@ -1319,7 +1325,8 @@ extern "C" int32_t tks_rope_append_paged_decode_mxfp4(
   // Every refusal of the attention comes before the append writes anything.
   if (max_seq_len < 0 || pages_per_split < 0 || num_kv_heads <= 0 || num_q_heads <= 0 ||
       num_q_heads % num_kv_heads != 0 || num_q_heads / num_kv_heads > kGenMaxG ||
-      block_size <= 0 || num_seqs < 0 || num_seqs > 65535 ||
+      block_size <= 0 || num_seqs < 0 || num_seqs > 65535 || num_blocks < 0 ||
+      !mx_rows_ok(num_blocks, num_kv_heads, block_size) ||
       ceil_div(max_seq_len, block_size) > block_table_stride)
     return valid_dtype(dtype) ? TKS_ERR_VALUE : TKS_ERR_TYPE;
   if (num_seqs > 0 && (!block_tables || !seq_lens || !out)) return TKS_ERR_VALUE;
@@ -1406,7 +1413,8 @@ extern "C" int32_t tks_paged_attention_prefill_mxfp4(
   if (!mx_pool_ok(num_layers, num_blocks, num_kv_heads, block_size, head_dim) || num_seqs < 0 ||
       num_tokens < 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads != 0 ||
       num_q_heads / num_kv_heads > kGenMaxG || max_query_len < 0 || max_seq_len < 0 ||
-      max_query_len > max_seq_len || block_table_stride < 0)
+      max_query_len > max_seq_len || block_table_stride < 0 ||
+      !mx_rows_ok(num_blocks, num_kv_heads, block_size))
     return TKS_ERR_VALUE;
   if (layer_index < 0 || layer_index >= num_layers) return TKS_ERR_INDEX;
   if (num_seqs == 0 || num_tokens == 0) return TKS_OK;
