@@ -53,7 +53,9 @@ __device__ __forceinline__ void tile_of(int64_t id, int64_t tiles_m, int64_t til
 // wait for it: unit_barrier waits, and nothing else in the loop counts as such a load.
 __device__ __forceinline__ void load_lds_async(const uint8_t *base, uint32_t off, uint32_t to) {
 #if __HIP_DEVICE_COMPILE__
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(to)
+  // (A wait state between the write of m0 and its use.)
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off),
+               "s"(base), "s"(to)
                : "memory", "m0");
 #else
   (void)base; (void)off; (void)to;
