@@ -503,7 +503,8 @@ int32_t tks_rope_kv_append_mxfp4(
 /* Decode attention: the function of tks_paged_attention_decode on the decoded pools
  * (exact values; scores exact products summed in fp32; probabilities of 8, 16 or 24
  * bits for bf16, fp16 and fp32 queries, summed in fp32). At most 16 query heads to a KV
- * head. A NaN block makes its outputs NaN where a query sees it. Workspace of tks_paged_attention_decode_workspace_bytes. */
+ * head. A NaN block makes its outputs NaN where a query sees it. Workspace of
+ * tks_paged_attention_decode_workspace_bytes. */
 int32_t tks_paged_attention_decode_mxfp4(
     const void *query, int64_t q_seq_stride, int64_t q_head_stride, const void *key_cache,
     const void *value_cache, const void *k_scales, const void *v_scales, int32_t num_layers,
@@ -514,8 +515,9 @@ int32_t tks_paged_attention_decode_mxfp4(
     int64_t out_head_stride, void *workspace, int64_t workspace_bytes, int32_t dtype,
     tks_stream_t stream);
 
-/* tks_rope_kv_append_mxfp4 then tks_paged_attention_decode_mxfp4, the rotated queries
- * staged in `out`. */
+/* tks_rope_kv_append_mxfp4 then tks_paged_attention_decode_mxfp4, in one launch where the
+ * rows are 16-byte aligned (else the rotated queries are staged in `out`). slot_mapping
+ * addresses position seq_lens[b] - 1; rows with a slot outside the pools are left out. */
 int32_t tks_rope_append_paged_decode_mxfp4(
     const void *query, int64_t q_seq_stride, int64_t q_head_stride, const void *key,
     int64_t k_seq_stride, int64_t k_head_stride, const void *value, int64_t v_seq_stride,

@@ -295,6 +295,49 @@ def test_rope_append_decode_is_its_parts(device, dtype, hq, hkv, dh, block_size)
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,hkv,dh,block_size,pages", [
+    (8, 2, 64, 16, 2), (4, 1, 128, 32, 0), (16, 1, 32, 16, 1), (6, 2, 96, 48, 0), (8, 8, 64, 5, 7)])
+def test_rope_append_decode_at_the_edges(device, dtype, hq, hkv, dh, block_size, pages) -> None:
+    """The new row first, last or alone in a tile and in a split, of sequences without keys, and
+    of rows that are not 16-byte aligned: the two calls' results bit for bit, pools included."""
+
+    lengths = [0, 1, 32, 33, 64, 65, 127, 128, 129, 320, 321, 2100]
+    n = len(lengths)
+    g = torch.Generator().manual_seed(12)
+    table = ops.RotaryTable(dh, theta=1e4, max_position=4000, dtype=dtype, device=device)
+    positions = torch.tensor([max(x - 1, 0) for x in lengths], device=device)
+    for shift in (0, 1):  # elements off the alignment
+        rows = []
+        for h in (hq, hkv, hkv):
+            flat = torch.randn(n * h * (dh + 8) + 1, generator=g).to(dtype).to(device)
+            rows.append(flat[shift:shift + n * h * (dh + 8)].view(n, h, dh + 8)[..., :dh])
+        query, key, value = rows
+        results = []
+        for fused in (True, False):
+            pool = Pool(lengths, hkv, dh, block_size, device, seed=6)
+            slots = _slots(pool, block_size, [max(x - 1, 0) for x in lengths], [1] * n).to(device)
+            slots[0] = -1
+            slots[6] = pool.key.shape[1] * block_size  # (past the pools: left out)
+            more = dict(layer_index=0, max_seq_len=2100, pages_per_split=pages, **pool.scales)
+            before = query.clone()
+            if fused:
+                out = ops.rope_append_paged_decode(query, key, value, positions, table, pool.key,
+                                                   pool.value, slots, pool.block_tables,
+                                                   pool.lens, **more)
+                assert torch.equal(query, before)
+            else:
+                q = ops.rope_kv_append(query.clone(), key, value, positions, table, pool.key,
+                                       pool.value, slots, 0, **pool.scales)
+                out = ops.paged_attention_decode(q, pool.key, pool.value, pool.block_tables,
+                                                 pool.lens, **more)
+            results.append([out] + [t.view(torch.uint8) for t in (pool.key, pool.value,
+                                                                  *pool.scales.values())])
+        for a, b in zip(*results):
+            assert torch.equal(a, b)
+        assert not results[0][0][0].any()
+
+
 # ------------------------------------------------------------------- prefill
 
 

@@ -21,7 +21,46 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 
-template <typename T, int NB, bool PAGED16>
+// The sequence's new K and V rows of a KV head, rotated and quantized, to `row` and their slot's
+// place in the pools: by the first threads, eight values each. False: they have no slot.
+template <typename T, int NB>
+__device__ __forceinline__ bool append_row(const MxDecodeArgs &a, int b, int kvh, const T *crow,
+                                           const T *srow, NewRow<NB> &row) {
+  constexpr int DH = 32 * NB;
+  const int E = row_threads(DH);
+  const MxDecodeRope &p = a.step;
+  const int64_t slot = p.slots[b];
+  if (slot < 0 || slot >= a.kc.num_blocks * a.kc.block_size) return false;
+  const int n = threadIdx.x, d = (n % E) * 8;
+  if (n < 2 * E && d < DH) {
+    const bool is_k = n < E;
+    const T *src = is_k ? static_cast<const T *>(p.k) + b * p.k_ss + kvh * p.k_hs
+                        : static_cast<const T *>(p.v) + b * p.v_ss + kvh * p.v_hs;
+    MxEight<T> x;
+    if (is_k)
+      x = rotated8<T, true>(src, crow, srow, d, DH / 2);
+    else
+      x = mx_load8<T>(src + d);
+    uint32_t s;
+    const uint32_t codes = mx_quantize<T>(x, &s);
+    const int64_t block = slot / a.kc.block_size;
+    const MxPool &pool = is_k ? a.kc : a.vc;
+    const int64_t at = pool.row(block, kvh, static_cast<int>(slot - block * a.kc.block_size));
+    *reinterpret_cast<uint32_t *>(pool.codes + at * (DH / 2) + d / 2) = codes;
+    *reinterpret_cast<uint32_t *>((is_k ? row.k : row.v) + d / 2) = codes;
+    if ((d & 31) == 0) {
+      pool.scales[at * NB + d / 32] = static_cast<uint8_t>(s);
+      (is_k ? row.ks : row.vs)[d / 32] = static_cast<uint8_t>(s);
+    }
+  }
+  return true;
+}
+
+// ROPE: a decode step (MxDecodeRope). The workgroup that holds the sequence's last key appends it
+// (of a sequence of no keys: the first), and attends to it from LDS, since what another workgroup
+// of the CU has in its L1 may be older. bf16, 4 KV heads of Dh 64, 512 keys, in a decode graph: 1.0
+// us less than with the append in a launch of its own for one sequence, 1.1 for 128.
+template <typename T, int NB, bool PAGED16, bool ROPE>
 __global__ __launch_bounds__(kThreads, 2) void decode_mx_kernel(MxDecodeArgs a) {
   constexpr int DH = 32 * NB;
   constexpr int J = 2 * NB;  // P.V products: 16 dims each
@@ -37,6 +76,18 @@ __global__ __launch_bounds__(kThreads, 2) void decode_mx_kernel(MxDecodeArgs a) 
   const int G = a.group;
   const int len = min(max(a.seq_lens[b], 0), a.key_cap);
   const int begin = split * a.split_keys;
+  const T *crow = nullptr, *srow = nullptr;
+  bool appended = false;
+  __shared__ NewRow<NB> new_row;
+  if constexpr (ROPE) {
+    const int64_t pos = min(max(a.step.positions[b], int64_t{0}), a.step.table_len - 1);
+    crow = static_cast<const T *>(a.step.cos_t) + pos * (DH / 2);
+    srow = static_cast<const T *>(a.step.sin_t) + pos * (DH / 2);
+    if (len > 0 ? begin < len && len - begin <= a.split_keys : split == 0) {
+      appended = append_row<T, NB>(a, b, kvh, crow, srow, new_row);
+      __syncthreads();
+    }
+  }
   T *out = static_cast<T *>(a.out) + b * a.o_ss + static_cast<int64_t>(kvh) * G * a.o_hs;
   if (begin >= len) {
     if (split == 0)
@@ -47,11 +98,14 @@ __global__ __launch_bounds__(kThreads, 2) void decode_mx_kernel(MxDecodeArgs a) 
   const int end = min(len, begin + a.split_keys);
   const int head = min(i, G - 1);  // (rows past the group: zeros)
   MxAttention<T, NB, PAGED16, false> at;
-  at.start(static_cast<const T *>(a.q) + b * a.q_ss +
-               (static_cast<int64_t>(kvh) * G + head) * a.q_hs + 8 * NB * g,
-           i < G, a.q_vec, a.scale_log2);
-  at.run(a.kc, a.vc, a.bt + static_cast<int64_t>(b) * a.bt_stride, kvh, begin, end, end, wave,
-         kWaves, lane);
+  const T *q = static_cast<const T *>(a.q) + b * a.q_ss +
+               (static_cast<int64_t>(kvh) * G + head) * a.q_hs;
+  if constexpr (ROPE)
+    at.start_rotated(q, crow, srow, g, i < G, a.scale_log2);
+  else
+    at.start(q + 8 * NB * g, i < G, a.q_vec, a.scale_log2);
+  at.run(a.kc, a.vc, a.bt + static_cast<int64_t>(b) * a.bt_stride, kvh, begin, end,
+         appended ? end - 1 : end, wave, kWaves, lane, appended ? &new_row : nullptr);
   const float l = xgroup_sum(at.l);
 
   if (g == 0) {
@@ -94,10 +148,15 @@ __global__ __launch_bounds__(kThreads, 2) void decode_mx_kernel(MxDecodeArgs a) 
 template <typename T, int NB>
 int32_t launch(const MxDecodeArgs &a, int32_t num_seqs, hipStream_t s) {
   const dim3 grid(a.kc.num_kv_heads, num_seqs, a.max_splits);
-  if (a.kc.block_size % 16 == 0)
-    decode_mx_kernel<T, NB, true><<<grid, kThreads, 0, s>>>(a);
+  const bool paged16 = a.kc.block_size % 16 == 0;
+  if (a.rope && paged16)
+    decode_mx_kernel<T, NB, true, true><<<grid, kThreads, 0, s>>>(a);
+  else if (a.rope)
+    decode_mx_kernel<T, NB, false, true><<<grid, kThreads, 0, s>>>(a);
+  else if (paged16)
+    decode_mx_kernel<T, NB, true, false><<<grid, kThreads, 0, s>>>(a);
   else
-    decode_mx_kernel<T, NB, false><<<grid, kThreads, 0, s>>>(a);
+    decode_mx_kernel<T, NB, false, false><<<grid, kThreads, 0, s>>>(a);
   return check_launch();
 }
 

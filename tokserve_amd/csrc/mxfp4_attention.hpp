@@ -25,6 +25,7 @@
 
 #include "attention_common.hpp"
 #include "mxfp4_kv.hpp"
+#include "mxfp4_rope.hpp"
 
 #include <type_traits>
 
@@ -138,6 +139,25 @@ __device__ __forceinline__ void load_v(const uint8_t *p, const uint8_t *s, uint3
     }
   }
 }
+// A row that is a sequence's last key, as it goes to the pools, in LDS.
+template <int NB>
+struct NewRow {
+  __align__(16) uint8_t k[16 * NB], v[16 * NB];
+  uint8_t ks[NB], vs[NB];
+};
+// It in place of key `in` of a loaded tile (lane (g, i), which holds key k_row of K).
+template <int NB>
+__device__ __forceinline__ void patch(Tile<NB> &t, const NewRow<NB> &row, int in, int g, int i,
+                                      int k_row) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (in >> 4 != h) continue;
+    if (k_row == (in & 15)) load_k<NB>(row.k, row.ks, 0, g, t.k[h], t.ks[h]);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (4 * r + g == (in & 15)) load_v<NB>(row.v, row.vs, 0, i, t.v[h][r], t.vs[h][r]);
+  }
+}
 // Output dim of A row i of P.V product jj.
 template <int NB>
 __device__ __forceinline__ int dim_of(int i, int jj) {
@@ -160,12 +180,28 @@ struct MxAttention {
   // scores' scale in log2 units. A negative one negates the queries, a zero one makes their
   // finite values zeros, so that row maxima are those of the raw scores.
   __device__ __forceinline__ void start(const T *row, bool live, bool vec, float scale_log2) {
-    const float sign = scale_log2 < 0.f ? -1.f : scale_log2 == 0.f ? 0.f : 1.f;
-    scale = scale_log2 == 0.f ? 1.f : fabsf(scale_log2);
     MxEight<T> raw[NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j)
       raw[j] = vec ? mx_load8<T>(row + 8 * j) : mx_load8_any<T>(row + 8 * j);
+    start(raw, live, scale_log2);
+  }
+  // The same of a row that starts at `row` (16-byte aligned as the others), rotated at the table
+  // rows c and s.
+  __device__ __forceinline__ void start_rotated(const T *row, const T *c, const T *s, int g,
+                                                bool live, float scale_log2) {
+    MxEight<T> raw[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      raw[j] = rotated8<T, true>(row, c, s, 8 * (NB * g + j), 16 * NB);
+      __builtin_amdgcn_sched_barrier(0);  // (one at a time: registers)
+    }
+    start(raw, live, scale_log2);
+  }
+  __device__ __forceinline__ void start(const MxEight<T> (&raw)[NB], bool live,
+                                        float scale_log2) {
+    const float sign = scale_log2 < 0.f ? -1.f : scale_log2 == 0.f ? 0.f : 1.f;
+    scale = scale_log2 == 0.f ? 1.f : fabsf(scale_log2);
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       float x[8];
@@ -292,10 +328,11 @@ struct MxAttention {
 
   // Keys [begin, end) of the sequence whose blocks bt lists, begin a multiple of 16: of their
   // tiles of 32 the wave takes number `first` and every `stride`-th after it. Every row sees
-  // those before `whole_end`.
+  // those before `whole_end`. With `last` (not null), key end - 1, at or behind `whole_end`, is
+  // that row.
   __device__ __forceinline__ void run(const MxPool &kc, const MxPool &vc, const int32_t *bt,
                                       int kvh, int begin, int end, int whole_end, int first,
-                                      int stride, int lane) {
+                                      int stride, int lane, const NewRow<NB> *last = nullptr) {
     const int g = lane >> 4, i = lane & 15;
     const int BS = kc.block_size;
     // Without PAGED16: rows (of this layer) of the keys of two of the wave's tiles, 2 pair and
@@ -395,6 +432,8 @@ struct MxAttention {
     }
     for (; n < mine; ++n) {
       if constexpr (CAUSAL) fetch(n + 1, odd);
+      if (!CAUSAL && last != nullptr && end - base_of(n) <= 32)
+        patch<NB>(even, *last, end - 1 - base_of(n), g, i, k_row);
       process(even, base_of(n), end, g, std::false_type{});
       if constexpr (CAUSAL) even = odd;
     }

@@ -72,8 +72,21 @@ struct MxPrefillArgs;
 int32_t launch_mx_marks(const MxPrefillArgs &a, const MxScratch &from, int32_t width,
                         int32_t dtype, hipStream_t s);
 
+// A decode step's new rows, one per sequence: its query rows are rotated at their positions,
+// the rotated K row and the V row quantized to their slots, the sequence's last key. All are
+// read 16 bytes at a time.
+struct MxDecodeRope {
+  const void *k, *v;
+  int64_t k_ss, k_hs, v_ss, v_hs;
+  const int64_t *positions, *slots;
+  const void *cos_t, *sin_t;
+  int64_t table_len;
+};
+
 // Decode attention over MXFP4 pools (decode_mxfp4.hip).
 struct MxDecodeArgs {
+  bool rope;
+  MxDecodeRope step;
   const void *q;
   int64_t q_ss, q_hs;
   bool q_vec;  // query rows can be read 16 bytes at a time

@@ -1234,7 +1234,8 @@ int32_t decode_mxfp4_impl(const void *query, int64_t q_seq_stride, int64_t q_hea
                           const int32_t *seq_order, int32_t num_seqs, int32_t num_q_heads,
                           int32_t max_seq_len, float scale, int32_t pages_per_split, void *out,
                           int64_t out_seq_stride, int64_t out_head_stride, void *workspace,
-                          int64_t workspace_bytes, int32_t dtype, tks_stream_t stream) {
+                          int64_t workspace_bytes, int32_t dtype, tks_stream_t stream,
+                          const MxDecodeRope *step = nullptr) {
   if (!valid_dtype(dtype)) return TKS_ERR_TYPE;
   if (!mx_pool_ok(num_layers, num_blocks, num_kv_heads, block_size, head_dim) || num_seqs < 0 ||
       num_q_heads <= 0 || num_q_heads % num_kv_heads != 0 || max_seq_len < 0 ||
@@ -1285,6 +1286,8 @@ int32_t decode_mxfp4_impl(const void *query, int64_t q_seq_stride, int64_t q_hea
   a.ws_m = w.m;
   a.ws_l = w.l;
   a.ws_acc = w.acc;
+  a.rope = step != nullptr;
+  if (step) a.step = *step;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int32_t st = launch_decode_mxfp4(a, dtype, num_seqs, s);
   if (st != TKS_OK || max_splits == 1) return st;
@@ -1322,6 +1325,27 @@ extern "C" int32_t tks_rope_append_paged_decode_mxfp4(
     int32_t num_seqs, int32_t num_q_heads, int32_t max_seq_len, float scale,
     int32_t pages_per_split, void *out, int64_t out_seq_stride, int64_t out_head_stride,
     void *workspace, int64_t workspace_bytes, int32_t dtype, tks_stream_t stream) {
+  if (valid_dtype(dtype) && num_seqs > 0 &&
+      (cache_len <= 0 || !key || !value || !positions || !cos_cache || !sin_cache ||
+       !slot_mapping))
+    return TKS_ERR_VALUE;
+  const int elem = elem_bytes(dtype);
+  auto rows16 = [&](const void *p, int64_t ss, int64_t hs) {
+    return aligned16(p) && ss * elem % 16 == 0 && hs * elem % 16 == 0;
+  };
+  if (rows16(query, q_seq_stride, q_head_stride) && rows16(key, k_seq_stride, k_head_stride) &&
+      rows16(value, v_seq_stride, v_head_stride) && aligned16(cos_cache) &&
+      aligned16(sin_cache)) {
+    const MxDecodeRope step{key,          value,         k_seq_stride, k_head_stride,
+                            v_seq_stride, v_head_stride, positions,    slot_mapping,
+                            cos_cache,    sin_cache,     cache_len};
+    return decode_mxfp4_impl(query, q_seq_stride, q_head_stride, key_cache, value_cache, k_scales,
+                             v_scales, num_layers, num_blocks, num_kv_heads, block_size, head_dim,
+                             layer_index, block_tables, block_table_stride, seq_lens, seq_order,
+                             num_seqs, num_q_heads, max_seq_len, scale, pages_per_split, out,
+                             out_seq_stride, out_head_stride, workspace, workspace_bytes, dtype,
+                             stream, &step);
+  }
   // Every refusal of the attention comes before the append writes anything.
   if (max_seq_len < 0 || pages_per_split < 0 || num_kv_heads <= 0 || num_q_heads <= 0 ||
       num_q_heads % num_kv_heads != 0 || num_q_heads / num_kv_heads > kGenMaxG ||

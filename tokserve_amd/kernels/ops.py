@@ -858,7 +858,7 @@ def rope_append_paged_decode(
     same arguments (one launch on the MFMA decode kernel; with per-row scales the append
     is a launch of its own ahead of the attention). Pools in the rows' dtype, or fp8
     pools with their scales (per pool, or per row with k_scales / v_scales), or MXFP4
-    pools with theirs (the append a launch of its own).
+    pools with theirs (one launch where the rows are 16-byte aligned).
     """
 
     require_hip("rope_append_paged_decode", query, key, value, positions, key_cache,
