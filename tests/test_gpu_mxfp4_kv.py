@@ -515,6 +515,58 @@ def test_refused_appends_and_gathers(device) -> None:
         assert not t.view(torch.uint8).any()
 
 
+def test_refused_attention(device) -> None:
+    """By the operators themselves, before anything is launched: out is as it was."""
+
+    pool = Pool([40, 3], 2, 64, 16, device, seed=4)
+    tables, lens = pool.block_tables, pool.lens
+    cu = torch.tensor([0, 1, 2], dtype=torch.int32, device=device)
+    query = torch.randn(2, 4, 64, device=device)
+    out = torch.full((2, 4, 64), 5.0, device=device)
+    base = dict(query=query, key_cache=pool.key, value_cache=pool.value, block_tables=tables,
+                seq_lens=lens, layer_index=0, max_seq_len=40, out=out, **pool.scales)
+    cases = [
+        (ValueError, "Hq, Dh\\) with the pool's Dh", dict(query=query[..., :32])),
+        (TypeError, "query must be float32", dict(query=query.double(), out=out.double())),
+        (ValueError, "divisible by KV head", dict(query=query[:, :3], out=out[:, :3])),
+        (ValueError, "out must match query", dict(out=out[:1])),
+        (ValueError, "out must match query", dict(out=out.half())),
+        (ValueError, "out must match query", dict(out=out.transpose(1, 2).contiguous().transpose(1, 2))),
+        (ValueError, "must match query", dict(block_tables=tables[:1])),
+        (ValueError, "must match query", dict(block_tables=tables[0])),
+        (TypeError, "block_tables must be torch.int32", dict(block_tables=tables.long())),
+        (TypeError, "seq_lens must be torch.int32", dict(seq_lens=lens.long())),
+        (ValueError, "seq_order must have shape", dict(seq_order=lens[:1])),
+        (TypeError, "seq_order must be torch.int32", dict(seq_order=lens.long())),
+        (ValueError, "requires HIP device", dict(seq_lens=lens.cpu())),
+        (ValueError, "requires HIP device", dict(query=query.cpu())),
+        (ValueError, "need k_scales", dict(k_scales=None, v_scales=None)),
+        (ValueError, "go together", dict(v_scales=None)),
+        (ValueError, "fp8 KV pools only", dict(k_scale=2.0)),
+        (IndexError, None, dict(layer_index=1)),
+        (ValueError, None, dict(max_seq_len=49)),
+    ]
+    for kind, match, change in cases:
+        for op in ("decode", "prefill"):
+            args = base | change
+            extra = dict(cu_seqlens_q=cu, max_query_len=1) if op == "prefill" else {}
+            with pytest.raises(kind, match=match):
+                getattr(ops, f"paged_attention_{op}")(**args, **extra)
+    with pytest.raises(ValueError, match="cu_seqlens_q"):
+        ops.paged_attention_prefill(**base, cu_seqlens_q=cu[:2], max_query_len=1)
+    with pytest.raises(ValueError, match="uint8"):
+        ops.paged_attention_decode(**base, workspace=torch.empty(8, device=device))
+    with pytest.raises(ValueError, match="workspace"):
+        ops.paged_attention_decode(**base, pages_per_split=1,
+                                   workspace=torch.empty(8, dtype=torch.uint8, device=device))
+    assert bool((out == 5).all())
+    # Strided queries are taken as they are.
+    wide = torch.randn(2, 4, 128, device=device)
+    again = ops.paged_attention_decode(**(base | dict(query=wide[..., ::2], out=None)))
+    assert torch.equal(again, ops.paged_attention_decode(
+        **(base | dict(query=wide[..., ::2].contiguous(), out=None))))
+
+
 # ------------------------------------------------------ the operators together
 
 

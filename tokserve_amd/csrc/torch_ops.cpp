@@ -172,6 +172,87 @@ Tensor scratch(int64_t bytes, const Tensor &query, const char *use) {
 }
 
 // Split partials of a decode: the caller's workspace, or scratch.
+// The MXFP4 matrix operators, and the cache's and the attention over MXFP4 pools, check their
+// arguments here (Python does the same for traced calls): there the checks of a small product
+// took 5 us of its 12.6, those of an append and a gather 11 of 21, of a decode 7 of 12.
+bool is_float(const Tensor &t) {
+  return t.scalar_type() == at::kFloat || t.scalar_type() == at::kHalf ||
+         t.scalar_type() == at::kBFloat16;
+}
+
+void one_device(const char *op, const Tensor &first, std::initializer_list<const Tensor *> others) {
+  TORCH_CHECK_VALUE(first.is_cuda(), op, " requires HIP device tensors");
+  for (const Tensor *t : others) {
+    if (t == nullptr) continue;
+    TORCH_CHECK_VALUE(t->is_cuda(), op, " requires HIP device tensors");
+    TORCH_CHECK_VALUE(t->device() == first.device(), op, ": tensors must use the same device");
+  }
+}
+
+const Tensor *maybe(const OptTensor &t) { return t ? &*t : nullptr; }
+
+void check_mxfp4_pools(const char *op, const Tensor &kc, const Tensor &vc,
+                       const OptTensor &k_scales, const OptTensor &v_scales) {
+  TORCH_CHECK_VALUE(kc.dim() == 5 && kc.sizes() == vc.sizes(),
+                    "KV pools must both have shape (L, NB, Hkv, BS, Dh)");
+  TORCH_CHECK_VALUE(kc.scalar_type() == vc.scalar_type(), "KV pools must use the same dtype");
+  TORCH_CHECK_VALUE(kc.is_contiguous() && vc.is_contiguous(), "KV pools must be contiguous");
+  const int64_t half = kc.size(4);
+  TORCH_CHECK_VALUE(half % 16 == 0 && half >= 16 && half <= 64,
+                    "MXFP4 KV pools need a head_dim of 32, 64, 96 or 128");
+  TORCH_CHECK_VALUE(k_scales || v_scales, op, ": MXFP4 KV pools need k_scales and v_scales");
+  TORCH_CHECK_VALUE(k_scales && v_scales, op, ": k_scales and v_scales go together");
+  for (const Tensor *t : {&*k_scales, &*v_scales}) {
+    const char *name = t == &*k_scales ? "k_scales" : "v_scales";
+    TORCH_CHECK_TYPE(t->scalar_type() == at::kFloat8_e8m0fnu, name,
+                     " of MXFP4 pools must be float8_e8m0fnu");
+    TORCH_CHECK_VALUE(t->dim() == 5 && t->sizes().slice(0, 4) == kc.sizes().slice(0, 4) &&
+                          t->size(4) == half / 16 && t->is_contiguous(),
+                      name, " must be a contiguous (L, NB, Hkv, BS, Dh / 32) tensor");
+  }
+}
+
+Tensor int_tensor(const Tensor &t, at::ScalarType type, const char *name) {
+  TORCH_CHECK_TYPE(t.scalar_type() == type, name, " must be torch.",
+                   type == at::kLong ? "int64" : "int32");
+  return t.contiguous();
+}
+
+// The arguments that decode and prefill share; query, tables, lengths and order as the kernels
+// take them.
+struct AttentionArgs {
+  Tensor query, tables, lens;
+  OptTensor order;
+};
+AttentionArgs check_mxfp4_attention(const char *op, const Tensor &query, const Tensor &kc,
+                                    const Tensor &vc, const Tensor &tables, const Tensor &lens,
+                                    const OptTensor &order, const Tensor &out,
+                                    const OptTensor &k_scales, const OptTensor &v_scales,
+                                    const Tensor *more, const char *rows) {
+  one_device(op, query, {&kc, &vc, &tables, &lens, maybe(order), &out, maybe(k_scales),
+                         maybe(v_scales), more});
+  check_mxfp4_pools(op, kc, vc, k_scales, v_scales);
+  TORCH_CHECK_VALUE(query.dim() == 3 && query.size(2) == 2 * kc.size(4), "query must have shape (",
+                    rows, ", Hq, Dh) with the pool's Dh");
+  TORCH_CHECK_TYPE(is_float(query), op, ": query must be float32, float16 or bfloat16");
+  TORCH_CHECK_VALUE(kc.size(2) > 0 && query.size(1) % kc.size(2) == 0,
+                    "query head count must be divisible by KV head count");
+  TORCH_CHECK_VALUE(out.sizes() == query.sizes() && out.scalar_type() == query.scalar_type() &&
+                        (out.numel() == 0 || out.stride(2) == 1),
+                    "out must match query and be contiguous in head_dim");
+  AttentionArgs r{query.stride(2) == 1 ? query : query.contiguous(),
+                  int_tensor(tables, at::kInt, "block_tables"),
+                  int_tensor(lens, at::kInt, "seq_lens"), order};
+  TORCH_CHECK_VALUE(tables.dim() == 2 && lens.dim() == 1 && lens.size(0) == tables.size(0),
+                    "block_tables (B, max_blocks) and seq_lens (B,) must match query");
+  if (order) {
+    r.order = int_tensor(*order, at::kInt, "seq_order");
+    TORCH_CHECK_VALUE(order->dim() == 1 && order->size(0) == lens.size(0),
+                      "seq_order must have shape (B,)");
+  }
+  return r;
+}
+
 Tensor decode_workspace(const OptTensor &given, const Tensor &query, const Tensor &pool,
                         int64_t max_seq_len, int64_t pages_per_split) {
   if (given) return *given;
@@ -181,13 +262,25 @@ Tensor decode_workspace(const OptTensor &given, const Tensor &query, const Tenso
                  query, "decode");
 }
 
-void paged_attention_decode(const Tensor &query, const Tensor &key_cache,
-                            const Tensor &value_cache, const Tensor &block_tables,
-                            const Tensor &seq_lens, const OptTensor &seq_order,
-                            int64_t layer_index, int64_t max_seq_len, double scale,
+void paged_attention_decode(const Tensor &q, const Tensor &key_cache,
+                            const Tensor &value_cache, const Tensor &tables,
+                            const Tensor &lens, const OptTensor &order, int64_t layer_index, int64_t max_seq_len, double scale,
                             int64_t pages_per_split, double k_scale, double v_scale,
                             const Tensor &out, const OptTensor &workspace,
                             const OptTensor &k_scales, const OptTensor &v_scales) {
+  AttentionArgs args{q, tables, lens, order};
+  if (mxfp4(key_cache)) {
+    const char *op = "paged_attention_decode";
+    args = check_mxfp4_attention(op, q, key_cache, value_cache, tables, lens, order, out, k_scales,
+                                 v_scales, maybe(workspace), "B");
+    TORCH_CHECK_VALUE(lens.size(0) == q.size(0),
+                      "block_tables (B, max_blocks) and seq_lens (B,) must match query");
+    TORCH_CHECK_VALUE(!workspace || (workspace->scalar_type() == at::kByte &&
+                                     workspace->is_contiguous()),
+                      "workspace must be a contiguous uint8 tensor");
+  }
+  const Tensor &query = args.query, &block_tables = args.tables, &seq_lens = args.lens;
+  const OptTensor &seq_order = args.order;
   const c10::DeviceGuard guard(query.device());
   const Library &l = library();
   const Tensor ws = decode_workspace(workspace, query, key_cache, max_seq_len, pages_per_split);
@@ -229,13 +322,24 @@ Tensor fp8_pages(const Tensor &query, const Tensor &pool, int64_t num_seqs, int6
                  query, "fp8 prefill");
 }
 
-void paged_attention_prefill(const Tensor &query, const Tensor &key_cache,
-                             const Tensor &value_cache, const Tensor &block_tables,
-                             const Tensor &seq_lens, const Tensor &cu_seqlens_q,
-                             const OptTensor &seq_order, int64_t layer_index,
+void paged_attention_prefill(const Tensor &q, const Tensor &key_cache,
+                             const Tensor &value_cache, const Tensor &tables,
+                             const Tensor &lens, const Tensor &cu, const OptTensor &order,
+                             int64_t layer_index,
                              int64_t max_query_len, int64_t max_seq_len, double scale,
                              double k_scale, double v_scale, const Tensor &out,
                              const OptTensor &k_scales, const OptTensor &v_scales) {
+  AttentionArgs args{q, tables, lens, order};
+  Tensor cu_seqlens_q = cu;
+  if (mxfp4(key_cache)) {
+    args = check_mxfp4_attention("paged_attention_prefill", q, key_cache, value_cache, tables,
+                                 lens, order, out, k_scales, v_scales, &cu, "N");
+    cu_seqlens_q = int_tensor(cu, at::kInt, "cu_seqlens_q");
+    TORCH_CHECK_VALUE(cu.dim() == 1 && cu.size(0) == lens.size(0) + 1,
+                      "block_tables (B, max_blocks), seq_lens (B,), cu_seqlens_q (B+1,)");
+  }
+  const Tensor &query = args.query, &block_tables = args.tables, &seq_lens = args.lens;
+  const OptTensor &seq_order = args.order;
   const c10::DeviceGuard guard(query.device());
   const Library &l = library();
   const Tensor &kc = key_cache;
@@ -369,52 +473,6 @@ void rope_kv_append_(const Tensor &query, const Tensor &key, const Tensor &value
                      const OptTensor &v_scales) {
   rope_kv_append(query, key, value, positions, cos, sin, key_cache, value_cache, slot_mapping,
                  layer_index, query, key_out, k_scale, v_scale, k_scales, v_scales);
-}
-
-// The MXFP4 matrix operators and the cache's over MXFP4 pools check their arguments here (Python
-// does the same for traced calls): there the checks of a small product took 5 us of its 12.6,
-// those of an append and a gather 11 of 21.
-bool is_float(const Tensor &t) {
-  return t.scalar_type() == at::kFloat || t.scalar_type() == at::kHalf ||
-         t.scalar_type() == at::kBFloat16;
-}
-
-void one_device(const char *op, const Tensor &first, std::initializer_list<const Tensor *> others) {
-  TORCH_CHECK_VALUE(first.is_cuda(), op, " requires HIP device tensors");
-  for (const Tensor *t : others) {
-    if (t == nullptr) continue;
-    TORCH_CHECK_VALUE(t->is_cuda(), op, " requires HIP device tensors");
-    TORCH_CHECK_VALUE(t->device() == first.device(), op, ": tensors must use the same device");
-  }
-}
-
-const Tensor *maybe(const OptTensor &t) { return t ? &*t : nullptr; }
-
-void check_mxfp4_pools(const char *op, const Tensor &kc, const Tensor &vc,
-                       const OptTensor &k_scales, const OptTensor &v_scales) {
-  TORCH_CHECK_VALUE(kc.dim() == 5 && kc.sizes() == vc.sizes(),
-                    "KV pools must both have shape (L, NB, Hkv, BS, Dh)");
-  TORCH_CHECK_VALUE(kc.scalar_type() == vc.scalar_type(), "KV pools must use the same dtype");
-  TORCH_CHECK_VALUE(kc.is_contiguous() && vc.is_contiguous(), "KV pools must be contiguous");
-  const int64_t half = kc.size(4);
-  TORCH_CHECK_VALUE(half % 16 == 0 && half >= 16 && half <= 64,
-                    "MXFP4 KV pools need a head_dim of 32, 64, 96 or 128");
-  TORCH_CHECK_VALUE(k_scales || v_scales, op, ": MXFP4 KV pools need k_scales and v_scales");
-  TORCH_CHECK_VALUE(k_scales && v_scales, op, ": k_scales and v_scales go together");
-  for (const Tensor *t : {&*k_scales, &*v_scales}) {
-    const char *name = t == &*k_scales ? "k_scales" : "v_scales";
-    TORCH_CHECK_TYPE(t->scalar_type() == at::kFloat8_e8m0fnu, name,
-                     " of MXFP4 pools must be float8_e8m0fnu");
-    TORCH_CHECK_VALUE(t->dim() == 5 && t->sizes().slice(0, 4) == kc.sizes().slice(0, 4) &&
-                          t->size(4) == half / 16 && t->is_contiguous(),
-                      name, " must be a contiguous (L, NB, Hkv, BS, Dh / 32) tensor");
-  }
-}
-
-Tensor int_tensor(const Tensor &t, at::ScalarType type, const char *name) {
-  TORCH_CHECK_TYPE(t.scalar_type() == type, name, " must be torch.",
-                   type == at::kLong ? "int64" : "int32");
-  return t.contiguous();
 }
 
 void kv_append(const Tensor &key_rows, const Tensor &value_rows, const Tensor &key_cache,

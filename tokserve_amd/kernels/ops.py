@@ -145,11 +145,17 @@ def _row_scales(
 
 
 def _natively_checked(pool: torch.Tensor, k_scale: float, v_scale: float) -> bool:
-    """Whether the cache's operators check a call themselves: over MXFP4 pools, on the device.
-    (Traced calls are checked in Python.)"""
+    """Whether the cache's and the attention's operators check a call themselves: over MXFP4
+    pools, on the device. (Traced calls are checked in Python.)"""
 
     return (pool.dtype == MXFP4_DTYPE and type(pool) is torch.Tensor and k_scale == 1.0
             and v_scale == 1.0 and pool.is_cuda and not torch.compiler.is_compiling())
+
+
+def _default_scale(query: torch.Tensor, scale: float | None) -> float:
+    if scale is None:
+        return 1.0 / sqrt(max(query.shape[-1], 1)) if query.ndim else 1.0
+    return float(scale)
 
 
 def _last_dim_contiguous(tensor: torch.Tensor, name: str) -> torch.Tensor:
@@ -360,6 +366,14 @@ def paged_attention_decode(
     k_scales / v_scales (their values exact whatever the query's dtype).
     """
 
+    if _natively_checked(key_cache, k_scale, v_scale) and query.is_cuda:
+        if out is None:
+            out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+        _ops.paged_attention_decode(query, key_cache, value_cache, block_tables, seq_lens,
+                                    seq_order, layer_index, max_seq_len,
+                                    _default_scale(query, scale), pages_per_split, 1.0, 1.0, out,
+                                    workspace, k_scales, v_scales)
+        return out
     require_hip("paged_attention_decode", query, key_cache, value_cache, block_tables, seq_lens)
     num_layers, num_blocks, num_kv_heads, block_size, head_dim = _pool_shape(
         key_cache, value_cache
@@ -463,6 +477,14 @@ def paged_attention_prefill(
     k_scales / v_scales.
     """
 
+    if _natively_checked(key_cache, k_scale, v_scale) and query.is_cuda:
+        if out is None:
+            out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+        _ops.paged_attention_prefill(query, key_cache, value_cache, block_tables, seq_lens,
+                                     cu_seqlens_q, seq_order, layer_index, max_query_len,
+                                     max_seq_len, _default_scale(query, scale), 1.0, 1.0, out,
+                                     k_scales, v_scales)
+        return out
     require_hip(
         "paged_attention_prefill", query, key_cache, value_cache, block_tables, seq_lens,
         cu_seqlens_q,
