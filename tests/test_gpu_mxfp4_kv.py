@@ -338,6 +338,27 @@ def test_rope_append_decode_at_the_edges(device, dtype, hq, hkv, dh, block_size,
         assert not results[0][0][0].any()
 
 
+def test_rope_append_decode_under_a_short_bound(device) -> None:
+    """max_seq_len below a sequence's length (48 of 100 keys): the two calls' results."""
+
+    pool_of = lambda: Pool([100, 20], 2, 64, 16, device, seed=3)  # noqa: E731
+    g = torch.Generator().manual_seed(4)
+    query, key, value = (torch.randn(2, h, 64, generator=g).to(device) for h in (4, 2, 2))
+    table = ops.RotaryTable(64, theta=1e4, max_position=200, dtype=torch.float32, device=device)
+    positions = torch.tensor([99, 19], device=device)
+    fused, apart = pool_of(), pool_of()
+    slots = _slots(fused, 16, [99, 19], [1, 1]).to(device)
+    out = ops.rope_append_paged_decode(query, key, value, positions, table, fused.key, fused.value,
+                                       slots, fused.block_tables, fused.lens, layer_index=0,
+                                       max_seq_len=48, **fused.scales)
+    q = ops.rope_kv_append(query.clone(), key, value, positions, table, apart.key, apart.value,
+                           slots, 0, **apart.scales)
+    want = ops.paged_attention_decode(q, apart.key, apart.value, apart.block_tables, apart.lens,
+                                      layer_index=0, max_seq_len=48, **apart.scales)
+    assert torch.equal(out, want)
+    assert torch.equal(fused.key.view(torch.uint8), apart.key.view(torch.uint8))
+
+
 # ------------------------------------------------------------------- prefill
 
 

@@ -84,7 +84,8 @@ __global__ __launch_bounds__(kThreads, 2) void decode_mx_kernel(MxDecodeArgs a) 
     crow = static_cast<const T *>(a.step.cos_t) + pos * (DH / 2);
     srow = static_cast<const T *>(a.step.sin_t) + pos * (DH / 2);
     if (len > 0 ? begin < len && len - begin <= a.split_keys : split == 0) {
-      appended = append_row<T, NB>(a, b, kvh, crow, srow, new_row);
+      // (Under a bound that cuts the sequence short the new row is not among the keys.)
+      appended = append_row<T, NB>(a, b, kvh, crow, srow, new_row) && a.seq_lens[b] <= a.key_cap;
       __syncthreads();
     }
   }
